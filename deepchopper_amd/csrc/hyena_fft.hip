@@ -40,8 +40,7 @@ __global__ __launch_bounds__(256) void fft_twiddle_kernel(float2* __restrict__ t
 __device__ __forceinline__ float2 cmul(float2 a, float2 b) {
   return make_float2(fmaf(a.x, b.x, -a.y * b.y), fmaf(a.x, b.y, a.y * b.x));
 }
-// two-lane fp32 vectors: the pointwise phases are written on these so that they compile to v_pk_* instructions
-// (left as scalar float2 code the SLP vectoriser packed the butterflies but none of the pointwise loops)
+// two-lane fp32 vectors, for the pointwise phases
 typedef float v2f __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ v2f V(float2 a) { return v2f{a.x, a.y}; }
 __device__ __forceinline__ float2 F(v2f a) { return make_float2(a.x, a.y); }
@@ -681,7 +680,7 @@ __global__ __launch_bounds__(Q * (1 << LOGN) / 16) void hyena_fftq_filter_kernel
 // (alpha = (1 - i w) / 2, beta = (1 + i w) / 2: Z[k] = alpha a + beta b, conj Z[M-k] = beta a + alpha b, u = conj(alpha) P Z[k] +
 //  conj(beta) Qc conj Z[M-k], v likewise with alpha and beta swapped; |alpha|^2 = (1 + s) / 2, |beta|^2 = (1 - s) / 2,
 //  conj(alpha) beta = i c / 2.)  A, A', B are built once per filter and size class, in double, with the inverse transform's
-// 1 / M folded in; the kernel's product phase is then 8 packed FMAs per pair with no twiddle, no halving and no conjugation
+// 1 / M folded in; the kernel's product phase is then 16 FMAs per pair with no twiddle, no halving and no conjugation
 // left (round 5: 59 instructions per pair, 470 of a thread's ~2 000).  Bin 0 (Y[0] and Y[M] are real and pair with each
 // other) keeps its own two real factors in A; the self-paired middle bin has B = 0.
 // coef layout per channel: A[0 .. M/2] | A'[0 .. M/2] | B[0 .. M/2]  (float2 each).
@@ -709,34 +708,19 @@ __global__ __launch_bounds__(256) void hyena_fft_pairmap_kernel(const float2* __
   out[2 * H + kk] = make_float2((float)(-cw * dy * inv_m), (float)(cw * dx * inv_m));  // i c (dx + i dy)
 }
 
-// Complex multiply-accumulate on packed fp32 with every swizzle and sign as an operand modifier of v_pk_fma_f32 (op_sel picks the
-// half of a source per result lane, neg_lo / neg_hi negate a source per lane): two instructions per complex product, no moves.
-// (Written as vector code hipcc built the rotated operand (-x.y, x.x) with a v_xor + v_mov per product: 7 of 20 instructions
-// of a pair.)   r = acc + a x:   lo = a.x x.x - a.y x.y + acc.x,   hi = a.x x.y + a.y x.x + acc.y
-#define DC_PK_FMA(dst, s0, s1, s2, mods) asm("v_pk_fma_f32 %0, %1, %2, %3 " mods : "=v"(dst) : "v"(s0), "v"(s1), "v"(s2))
+// Complex multiply-accumulate, two FMAs per lane in a fixed order.   r = acc + a x:   lo = a.x x.x - a.y x.y + acc.x,
+// hi = a.x x.y + a.y x.x + acc.y
 __device__ __forceinline__ v2f pm_mul(v2f a, v2f x) {  // a x
-  v2f r;
-  asm("v_pk_mul_f32 %0, %1, %2 op_sel_hi:[0,1]" : "=v"(r) : "v"(a), "v"(x));  // a.xx * x
-  DC_PK_FMA(r, a, x, r, "op_sel:[1,1,0] op_sel_hi:[1,0,1] neg_lo:[0,1,0]");     // + a.yy * (-x.y, x.x)
-  return r;
+  return v2f{__builtin_fmaf(a.y, -x.y, a.x * x.x), __builtin_fmaf(a.y, x.x, a.x * x.y)};
 }
 __device__ __forceinline__ v2f pm_nmul(v2f a, v2f x) {  // -(a x)
-  v2f r;
-  asm("v_pk_mul_f32 %0, %1, %2 op_sel_hi:[0,1] neg_lo:[1,0] neg_hi:[1,0]" : "=v"(r) : "v"(a), "v"(x));
-  DC_PK_FMA(r, a, x, r, "op_sel:[1,1,0] op_sel_hi:[1,0,1] neg_hi:[0,1,0]");
-  return r;
+  return v2f{__builtin_fmaf(a.y, x.y, -(a.x * x.x)), __builtin_fmaf(a.y, -x.x, -(a.x * x.y))};
 }
 __device__ __forceinline__ v2f pm_fma_conj(v2f cm, v2f x, v2f acc) {  // acc + conj(cm) x
-  v2f r;
-  DC_PK_FMA(r, cm, x, acc, "op_sel_hi:[0,1,1]");                                  // + cm.xx * x
-  DC_PK_FMA(r, cm, x, r, "op_sel:[1,1,0] op_sel_hi:[1,0,1] neg_hi:[0,1,0]");      // - cm.yy * (-x.y, x.x)
-  return r;
+  return v2f{__builtin_fmaf(cm.y, x.y, __builtin_fmaf(cm.x, x.x, acc.x)), __builtin_fmaf(cm.y, -x.x, __builtin_fmaf(cm.x, x.y, acc.y))};
 }
-__device__ __forceinline__ v2f pm_fma_conj_out_conj(v2f cm, v2f x, v2f acc) {  // conj(acc + conj(cm) x): the last step negates its hi lane
-  v2f r;
-  DC_PK_FMA(r, cm, x, acc, "op_sel_hi:[0,1,1]");
-  DC_PK_FMA(r, cm, x, r, "op_sel:[1,1,0] op_sel_hi:[1,0,1] neg_hi:[0,0,1]");      // hi: -(-cm.y x.x + r.y) = cm.y x.x - r.y
-  return r;
+__device__ __forceinline__ v2f pm_fma_conj_out_conj(v2f cm, v2f x, v2f acc) {  // conj(acc + conj(cm) x)
+  return v2f{__builtin_fmaf(cm.y, x.y, __builtin_fmaf(cm.x, x.x, acc.x)), __builtin_fmaf(cm.y, x.x, -__builtin_fmaf(cm.x, x.y, acc.y))};
 }
 
 template <int LOGN, int Q, bool TAB, int SP, bool PM>
@@ -979,7 +963,7 @@ __global__ __launch_bounds__(Q * (1 << LOGN) / 16, 4) void hyena_fftq_kernel(Hye
 
   fft_lds<LOGN>(s + grp * ROW, tw, tid - grp * TG);
   // (opaque copies: left alone, hipcc keeps the NJ (Q - 1) products wb W_16^(j k1) of the forward step alive -- spilled --
-  //  across both transforms to reuse them below; recomputing them is a dozen packed multiplies)
+  //  across both transforms to reuse them below; recomputing them is a dozen complex multiplies)
 #pragma unroll
   for (int k1 = 1; k1 < Q; ++k1) asm volatile("" : "+v"(wb[k1].x), "+v"(wb[k1].y));
 
