@@ -103,6 +103,17 @@ _SIGNATURES = {
     "dc_model_profile_reset": (C.c_int, [vp]),
     "dc_model_profile_get": (C.c_int, [vp, C.c_char_p, C.POINTER(C.c_double), C.POINTER(i64)]),
     "dc_model_profile_stages": (C.c_int, [vp, C.c_char_p, i32]),
+    "dc_token_logprobs": (C.c_int, [vp, vp, i32, i64, i32, i64, vp, i32, i64, i32, vp, vp, vp, vp, vp, vp, i64]),
+    "dc_token_logprobs_workspace": (i64, [i64, i32, i32]),
+    "dc_token_logprobs_backward": (C.c_int, [vp, vp, i32, i64, i32, i64, vp, i32, i64, vp, vp, vp, vp, i64]),
+    "dc_gated_scan": (C.c_int, [vp, i32, vp, i64, vp, i64, i64, i32, vp, vp, i32, i64, i32, vp, vp, i64, i32, vp, vp, vp, i64]),
+    "dc_gated_scan_workspace": (i64, [i64, i32, i32, i64]),
+    "dc_gated_scan_saved": (i64, [i64, i32]),
+    "dc_gated_scan_backward": (C.c_int, [vp, i32, vp, i64, vp, i64, i64, i32, vp, vp, i32, i64, i32, vp, vp, vp, i64, vp, vp, i64, vp, i64, i32, vp, vp, i64]),
+    "dc_block_norm": (C.c_int, [vp, i32, i32, i64, i32, i32, C.c_float, vp, i64, vp, i64, i32, vp, i64, vp, i32, vp, vp, vp, vp, vp, i64, vp, i64]),
+    "dc_block_norm_backward": (C.c_int, [vp, i32, i32, i64, i32, i32, C.c_float, vp, i64, vp, i64, i32, vp, i64, vp, i32, vp, vp, vp, vp, i64, vp, i64,
+                                         vp, vp, vp, vp, vp, vp, vp, vp, vp, i64]),
+    "dc_block_norm_workspace": (i64, [i64, i32]),
 }
 
 _lib = None

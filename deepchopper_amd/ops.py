@@ -5,6 +5,7 @@ copies.  All arithmetic happens inside libdeepchopper_hip.so.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -187,6 +188,267 @@ def summary_predict_dense(pred: torch.Tensor, labels: torch.Tensor, ignore_label
     _lib.check(L.dc_summary_predict(_stream(), _ptr(pred), _ptr(labels), n_rows, row_stride, ignore_label, _ptr(offs),
                                     _ptr(op), _ptr(ol), _ptr(counts)))
     return op, ol, offs
+
+
+# ------------------------------------------------------------------------------------------
+# sequence-layer and scoring operators
+# ------------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_TOKEN_TYPES = {torch.int8: 0, torch.uint8: 1, torch.int32: 2, torch.int64: 3}
+_NORM_KINDS = {"layer": 0, "rms": 1}
+_GATE_ACTS = {"identity": 0, "sigmoid": 1, "silu": 2}
+STATS_FROM = 513  # DC_STATS_FROM: classes from which token_logprobs_backward needs the forward's statistics
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def _on(t: torch.Tensor):
+    """Context in which `t`'s device is the current one (a call's kernels run on ITS device's current stream)."""
+    i = t.device.index
+    return _NO_SWITCH if i == torch.cuda.current_device() else torch.cuda.device(i)
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _like(ref: torch.Tensor, name: str, t: torch.Tensor | None, shape, dtype: torch.dtype) -> int | None:
+    """Address of the contiguous tensor `t` (or None) after checking it against what the call needs."""
+    if t is None:
+        return None
+    _need(t.device == ref.device and t.dtype == dtype and t.shape == tuple(shape) and t.is_contiguous(),
+          f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on {ref.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _rows(ref: torch.Tensor, name: str, t: torch.Tensor | None, shape=None, dtype: torch.dtype | None = None) -> tuple[int | None, int]:
+    """(address, elements between rows) of a [..., width] tensor whose rows are contiguous and evenly spaced (the halves of
+    a projection, an expanded row), after checking it against `ref`'s device and the shape and type the call needs."""
+    if t is None:
+        return None, 0
+    _need(t.is_cuda and t.device == ref.device, f"{name}: device-resident tensor on {ref.device} required, got {t.device}")
+    _need(shape is None or t.shape == shape, f"{name}: expected shape {tuple(shape or ())}, got {tuple(t.shape)}")
+    _need(t.dtype == dtype if dtype is not None else t.dtype in _DTYPES, f"{name}: {t.dtype} is not {dtype or 'float32, float16 or bfloat16'}")
+    _need(t.dim() >= 2, f"{name}: at least two dimensions required, got {t.dim()}")
+    size, st = t.shape, t.stride()
+    _need(st[-1] == 1 or size[-1] <= 1 or t.numel() == 0, f"{name}: the last dimension must be contiguous")
+    # leading dimensions of size 1 say nothing about the distance of two rows
+    dims = [(n, s) for n, s in zip(size[:-1], st[:-1]) if n != 1]
+    if t.numel():
+        for (_, outer), (n, s) in zip(dims, dims[1:]):
+            _need(outer == n * s, f"{name}: rows must be evenly spaced (shape {tuple(size)}, strides {st})")
+    return t.data_ptr(), dims[-1][1] if dims else size[-1]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, n_top: int = 0, ignore_index: int = -100,
+                   want_entropy: bool = True, save: bool = False) -> dict:
+    """Log probability of a given token per row of logits [..., n_classes], the row's entropy and its `n_top` likeliest
+    classes (`dc_token_logprobs`).  `tokens` [...] int8 / uint8 / int32 / int64 or None; rows whose token is `ignore_index`
+    (labels of padding) are not read and give 0, alternatives -1.  Returns dict(logprob f32 or None, entropy f32 or None,
+    top_ids i32, top_logprob f32 [..., n_top] or None, stats: what `token_logprobs_backward` needs (with `save`; None below STATS_FROM
+    classes))."""
+    ptr, stride = _rows(logits, "logits", logits)
+    lead, n_classes = logits.shape[:-1], logits.shape[-1]
+    n = logits.numel() // max(n_classes, 1)
+    dev = logits.device
+    _need(tokens is None or tokens.dtype in _TOKEN_TYPES, "tokens: int8, uint8, int32 or int64 required")
+    tok = None if tokens is None else _like(logits, "tokens", tokens, lead, tokens.dtype)
+    logprob = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev) if want_entropy else None
+    stats = torch.empty((n, 3), dtype=torch.float32, device=dev) if save and n_classes >= STATS_FROM else None
+    ids = torch.empty((*lead, n_top), dtype=torch.int32, device=dev) if n_top > 0 else None
+    top = torch.empty((*lead, n_top), dtype=torch.float32, device=dev) if n_top > 0 else None
+    L = _lib.lib()
+    with _on(logits):
+        nb = L.dc_token_logprobs_workspace(n, n_classes, n_top)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        _lib.check(L.dc_token_logprobs(
+            _stream(), ptr, _DTYPES[logits.dtype], n, n_classes, stride, tok, 0 if tokens is None else _TOKEN_TYPES[tokens.dtype], ignore_index,
+            n_top, _ptr(logprob), _ptr(entropy), _ptr(stats), _ptr(ids), _ptr(top), _ptr(ws), nb))
+    return {"logprob": logprob, "entropy": entropy, "top_ids": ids, "top_logprob": top, "stats": stats}
+
+
+def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor | None, stats: torch.Tensor | None, grad_logprob: torch.Tensor | None,
+                            grad_entropy: torch.Tensor | None = None, *, ignore_index: int = -100) -> torch.Tensor:
+    """Gradient of the logits for gradients of `token_logprobs`' logprob and entropy (either None: zero); `stats` as it
+    returned them with `save=True`."""
+    ptr, stride = _rows(logits, "logits", logits)
+    lead, n_classes = logits.shape[:-1], logits.shape[-1]
+    n = logits.numel() // max(n_classes, 1)
+    _need(tokens is None or tokens.dtype in _TOKEN_TYPES, "tokens: int8, uint8, int32 or int64 required")
+    tok = None if tokens is None else _like(logits, "tokens", tokens, lead, tokens.dtype)
+    st = _like(logits, "stats", stats, (n, 3), torch.float32)
+    gl = _like(logits, "grad_logprob", grad_logprob, lead, torch.float32)
+    gh = _like(logits, "grad_entropy", grad_entropy, lead, torch.float32)
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    with _on(logits):
+        _lib.check(_lib.lib().dc_token_logprobs_backward(
+            _stream(), ptr, _DTYPES[logits.dtype], n, n_classes, stride, tok, 0 if tokens is None else _TOKEN_TYPES[tokens.dtype], ignore_index, st,
+            gl, gh, out.data_ptr(), n_classes))
+    return out
+
+
+def _scan_shape(x: torch.Tensor, offsets, begin, end, max_len):
+    """(tokens, channels, sequences, longest, address of begin, of end) of a gated_scan call."""
+    if offsets is None and begin is None and end is None:
+        _need(x.dim() == 3, "x: [n_seqs, length, n_channels] required without offsets")
+        _need(max_len is None or max_len == x.shape[1], "max_len of dense sequences is their length")
+        return x.shape[0] * x.shape[1], x.shape[2], x.shape[0], x.shape[1], None, None
+    _need((offsets is None) == (begin is not None) and (begin is None) == (end is None), "either offsets, or begin and end")
+    if offsets is not None:
+        _need(offsets.dim() == 1 and offsets.numel() >= 1, "offsets: int64[n_seqs + 1] required")
+        n = offsets.numel() - 1
+        b = _like(x, "offsets", offsets, (n + 1,), torch.int64)
+        e = b + 8
+    else:
+        n = begin.numel()
+        b, e = _like(x, "begin", begin, (n,), torch.int64), _like(x, "end", end, (n,), torch.int64)
+    if max_len is None:  # read back: callers that know the longest sequence pass it (and need to inside a graph capture)
+        lens = offsets.diff() if offsets is not None else end - begin
+        max_len = max(int(lens.max().item()), 0) if n else 0
+    return x.numel() // max(x.shape[-1], 1), x.shape[-1], n, int(max_len), b, e
+
+
+def gated_scan(x: torch.Tensor, f: torch.Tensor, *, offsets: torch.Tensor | None = None, begin: torch.Tensor | None = None,
+               end: torch.Tensor | None = None, max_len: int | None = None, h0: torch.Tensor | None = None, reverse: bool = False,
+               save: bool = False, out: torch.Tensor | None = None, h_last: torch.Tensor | None = None) -> dict:
+    """h_t = sigmoid(f_t) h_(t-1) + (1 - sigmoid(f_t)) x_t along every sequence, per channel (`dc_gated_scan`): the recurrent
+    counterpart of the long convolution, for reads of any length, with a state to carry on with.
+
+    x, f [n_seqs, length, n_channels] dense, or [n_tokens, n_channels] with the sequences at `offsets` int64[n_seqs + 1], or at
+    `begin` / `end` int64[n_seqs] (left-padded rows: first column and end of each).  `h0` f32[n_seqs, n_channels] state to start from; `reverse`: from
+    the sequences' ends.  `h_last` may be given (`h0` itself: a state kept in place while bases stream in); `out` keeps what stands in
+    tokens of no sequence, which are zero otherwise.  Returns dict(y, h_last, saved: for `gated_scan_backward`, with `save`)."""
+    xp, xs = _rows(x, "x", x)
+    fp, fs = _rows(x, "f", f, x.shape, x.dtype)
+    n, c, seqs, longest, b, e = _scan_shape(x, offsets, begin, end, max_len)
+    dev = x.device
+    h0p = _like(x, "h0", h0, (seqs, c), torch.float32)
+    zero_rest = out is None and offsets is not None  # (dense sequences cover every token)
+    if out is None:
+        out = (torch.empty if begin is None else torch.zeros)(x.shape, dtype=x.dtype, device=dev)
+    yp, ys = _rows(x, "out", out, x.shape, x.dtype)
+    if h_last is None:
+        h_last = torch.empty((seqs, c), dtype=torch.float32, device=dev)
+    hp = _like(x, "h_last", h_last, (seqs, c), torch.float32)
+    L = _lib.lib()
+    saved = torch.empty(L.dc_gated_scan_saved(n, c), dtype=torch.float32, device=dev) if save else None
+    with _on(x):
+        nb = L.dc_gated_scan_workspace(n, c, seqs, longest)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        _lib.check(L.dc_gated_scan(_stream(), _DTYPES[x.dtype], xp, xs, fp, fs, n, c, b, e, seqs, longest, int(reverse), h0p, yp, ys, int(zero_rest),
+                                   hp, _ptr(saved), _ptr(ws), nb))
+    return {"y": out, "h_last": h_last, "saved": saved}
+
+
+def gated_scan_backward(x: torch.Tensor, f: torch.Tensor, saved: torch.Tensor, grad_y: torch.Tensor, *, grad_h_last: torch.Tensor | None = None,
+                        h0: torch.Tensor | None = None, offsets: torch.Tensor | None = None, begin: torch.Tensor | None = None,
+                        end: torch.Tensor | None = None, max_len: int | None = None, reverse: bool = False) -> dict:
+    """Gradients of `gated_scan` for `grad_y` (and `grad_h_last`): dict(grad_x, grad_f, grad_h0 f32[n_seqs, n_channels]).  The other
+    arguments as in the forward call, `saved` as it returned it; tokens of no sequence get zeros."""
+    xp, xs = _rows(x, "x", x)
+    fp, fs = _rows(x, "f", f, x.shape, x.dtype)
+    gp, gs = _rows(x, "grad_y", grad_y, x.shape, x.dtype)
+    n, c, seqs, longest, b, e = _scan_shape(x, offsets, begin, end, max_len)
+    dev = x.device
+    L = _lib.lib()
+    h0p = _like(x, "h0", h0, (seqs, c), torch.float32)
+    glp = _like(x, "grad_h_last", grad_h_last, (seqs, c), torch.float32)
+    sp = _like(x, "saved", saved, (L.dc_gated_scan_saved(n, c),), torch.float32)
+    make = torch.empty if begin is None else torch.zeros
+    gx, gf = make(x.shape, dtype=x.dtype, device=dev), make(x.shape, dtype=x.dtype, device=dev)
+    gh = torch.empty((seqs, c), dtype=torch.float32, device=dev)
+    with _on(x):
+        nb = L.dc_gated_scan_workspace(n, c, seqs, longest)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        _lib.check(L.dc_gated_scan_backward(_stream(), _DTYPES[x.dtype], xp, xs, fp, fs, n, c, b, e, seqs, longest, int(reverse), h0p, sp, gp, gs,
+                                            glp, gx.data_ptr(), c, gf.data_ptr(), c, int(offsets is not None), gh.data_ptr(), _ptr(ws), nb))
+    return {"grad_x": gx, "grad_f": gf, "grad_h0": gh}
+
+
+def _norm_ref(y, residual) -> torch.Tensor:
+    ref = y if y is not None else residual
+    _need(ref is not None, "block_norm: a block's output or a residual is required")
+    return ref
+
+
+def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None = None, gate: torch.Tensor | None = None, *, kind: str = "layer",
+               gate_act: str = "sigmoid", scale: torch.Tensor | None = None, post: bool = True, post_weight: torch.Tensor | None = None,
+               post_bias: torch.Tensor | None = None, pre: bool = True, pre_weight: torch.Tensor | None = None, pre_bias: torch.Tensor | None = None,
+               eps: float = 1e-5, dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> dict:
+    """What stands between two blocks, in one pass (`dc_block_norm`): r' = residual + scale * act(gate) * norm(y) and n = norm(r').
+
+    y, gate [..., width] of one type, residual of that type or float32.  `post=False`: no norm behind the block; `pre=False`: none in
+    front of the next (the last block); y None: the first norm of a model; residual None: r' is the block's output alone.  Norms are
+    "layer" or "rms", gates "identity", "sigmoid" or "silu"; weights, biases and `scale` are float32[width].  `dtype`: of n where y is
+    None (default: the residual's); `out`: where r' goes (`residual` itself: in place).  Returns dict(residual: r', normed: n or None)."""
+    ref = _norm_ref(y, residual)
+    _need(kind in _NORM_KINDS, f"kind: one of {sorted(_NORM_KINDS)}")
+    _need(gate_act in _GATE_ACTS, f"gate_act: one of {sorted(_GATE_ACTS)}")
+    act_dtype = y.dtype if y is not None else dtype or ref.dtype
+    res_dtype = residual.dtype if residual is not None else act_dtype
+    _need(act_dtype in _DTYPES, f"{act_dtype} is not float32, float16 or bfloat16")
+    _need(gate is None or y is not None, "gate: without a block's output")
+    shape, w = ref.shape, ref.shape[-1]
+    yp, ys = _rows(ref, "y", y, shape)
+    gp, gs = _rows(ref, "gate", gate, shape, act_dtype)
+    rp, rs = _rows(ref, "residual", residual, shape)
+    vec = [_like(ref, n, t, (w,), torch.float32) for n, t in (("scale", scale), ("post_weight", post_weight), ("post_bias", post_bias),
+                                                            ("pre_weight", pre_weight), ("pre_bias", pre_bias))]
+    if out is None and y is not None:
+        out = torch.empty(shape, dtype=res_dtype, device=ref.device)
+    op, os_ = _rows(ref, "out", out, shape, res_dtype)
+    normed = torch.empty(shape, dtype=act_dtype, device=ref.device) if pre else None
+    with _on(ref):
+        _lib.check(_lib.lib().dc_block_norm(
+            _stream(), _DTYPES[act_dtype], _DTYPES.get(res_dtype, -1), ref.numel() // max(w, 1), w, _NORM_KINDS[kind], eps, yp, ys, gp, gs,
+            _GATE_ACTS[gate_act], rp, rs, vec[0], int(post), vec[1], vec[2], vec[3], vec[4], op, os_, _ptr(normed), w))
+    return {"residual": residual if out is None else out, "normed": normed}
+
+
+def block_norm_backward(y: torch.Tensor | None, residual: torch.Tensor | None = None, gate: torch.Tensor | None = None, *,
+                        grad_residual: torch.Tensor | None = None, grad_normed: torch.Tensor | None = None, kind: str = "layer",
+                        gate_act: str = "sigmoid", scale: torch.Tensor | None = None, post: bool = True,
+                        post_weight: torch.Tensor | None = None, post_bias: torch.Tensor | None = None, pre_weight: torch.Tensor | None = None,
+                        pre_bias: torch.Tensor | None = None, eps: float = 1e-5) -> dict:
+    """Gradients of `block_norm` for gradients of r' (`grad_residual`) and n (`grad_normed`), either None where it is not used.  The other
+    arguments as in the forward call, `residual` as it was BEFORE it.  Returns dict(grad_y, grad_gate, grad_residual, and float32[width]
+    grad_scale, grad_post_weight, grad_post_bias, grad_pre_weight, grad_pre_bias); None for what the call did not have."""
+    ref = _norm_ref(y, residual)
+    _need(kind in _NORM_KINDS, f"kind: one of {sorted(_NORM_KINDS)}")
+    _need(gate_act in _GATE_ACTS, f"gate_act: one of {sorted(_GATE_ACTS)}")
+    act_dtype = y.dtype if y is not None else grad_normed.dtype if grad_normed is not None else ref.dtype
+    res_dtype = residual.dtype if residual is not None else act_dtype
+    _need(act_dtype in _DTYPES, f"{act_dtype} is not float32, float16 or bfloat16")
+    _need(gate is None or y is not None, "gate: without a block's output")
+    shape, w, dev = ref.shape, ref.shape[-1], ref.device
+    n = ref.numel() // max(w, 1)
+    yp, ys = _rows(ref, "y", y, shape)
+    gp, gs = _rows(ref, "gate", gate, shape, act_dtype)
+    rp, rs = _rows(ref, "residual", residual, shape)
+    grp, grs = _rows(ref, "grad_residual", grad_residual, shape, res_dtype)
+    gnp, gns = _rows(ref, "grad_normed", grad_normed, shape, act_dtype)
+    vec = [_like(ref, m, t, (w,), torch.float32) for m, t in (("scale", scale), ("post_weight", post_weight), ("post_bias", post_bias),
+                                                            ("pre_weight", pre_weight))]
+    _like(ref, "pre_bias", pre_bias, (w,), torch.float32)
+
+    def grad(like, dt=torch.float32):
+        return None if like is None else torch.empty(like.shape, dtype=dt, device=dev)
+
+    normed = post and y is not None
+    g = {"grad_y": grad(y, act_dtype), "grad_gate": grad(gate, act_dtype), "grad_residual": grad(residual, res_dtype),
+         "grad_scale": grad(scale) if y is not None else None, "grad_post_weight": grad(post_weight) if normed else None,
+         "grad_post_bias": grad(post_bias) if normed else None, "grad_pre_weight": grad(pre_weight), "grad_pre_bias": grad(pre_bias)}
+    L = _lib.lib()
+    with _on(ref):
+        nb = L.dc_block_norm_workspace(n, w)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        _lib.check(L.dc_block_norm_backward(
+            _stream(), _DTYPES[act_dtype], _DTYPES.get(res_dtype, -1), n, w, _NORM_KINDS[kind], eps, yp, ys, gp, gs, _GATE_ACTS[gate_act], rp, rs,
+            vec[0], int(post), vec[1], vec[2], vec[3], grp, grs, gnp, gns, _ptr(g["grad_y"]), _ptr(g["grad_gate"]), _ptr(g["grad_residual"]),
+            _ptr(g["grad_scale"]), _ptr(g["grad_post_weight"]), _ptr(g["grad_post_bias"]), _ptr(g["grad_pre_weight"]), _ptr(g["grad_pre_bias"]),
+            _ptr(ws), nb))
+    return g
 
 
 # ------------------------------------------------------------------------------------------

@@ -387,6 +387,129 @@ int dc_model_profile_get(dc_model* m, const char* stage, double* total_ms, int64
 /* comma-separated list of the stages recorded so far */
 int dc_model_profile_stages(dc_model* m, char* buf, int32_t buf_len);
 
+/* ------------------------------------------------------------------------------------------
+ * Sequence-layer and scoring operators
+ *
+ * What stands beside the model handle for callers that build, train or score a layer themselves: the recurrent counterpart
+ * of the long convolution, the norms / gate / residual between two blocks, and the probabilities behind the logits that
+ * the smoothing path reduces to labels.  Common conventions, on top of those at the top of this file:
+ *  - element types are DC_DTYPE_*; states, statistics, weights and their gradients are fp32; everything is computed in fp32
+ *    and rounded once, to nearest even, where an output is DC_DTYPE_F16 / DC_DTYPE_BF16;
+ *  - a row (token) is contiguous; *_stride is the distance of two rows in ELEMENTS (inputs: >= 0, 0 repeats one row;
+ *    outputs: >= the row's width), so the halves of one projection are passed as they lie; outputs without a stride
+ *    argument are dense;
+ *  - pointers marked "or NULL" may be NULL; element pointers are aligned to their element;
+ *  - the result of a call goes by its inputs alone (no atomics: the same call gives the same bits);
+ *  - workspaces are caller-owned scratch of at least the size the *_workspace function gives for the same sizes (0: NULL is
+ *    fine), 16-byte aligned, free for reuse as soon as the call's kernels have run;
+ *  - nothing is allocated, cleared or synchronised inside a call: every entry point may be captured into a graph.
+ * ------------------------------------------------------------------------------------------ */
+#define DC_DTYPE_F32 0
+#define DC_DTYPE_F16 1
+#define DC_DTYPE_BF16 2
+#define DC_TOKENS_I8 0
+#define DC_TOKENS_U8 1
+#define DC_TOKENS_I32 2
+#define DC_TOKENS_I64 3
+#define DC_NORM_LAYER 0
+#define DC_NORM_RMS 1
+#define DC_ACT_IDENTITY 0
+#define DC_ACT_SIGMOID 1
+#define DC_ACT_SILU 2
+#define DC_MAX_TOP 32            /* most alternatives dc_token_logprobs reports                              */
+#define DC_MAX_NORM_WIDTH 16384  /* widest row of dc_block_norm                                              */
+#define DC_STATS_FROM 513        /* classes from which dc_token_logprobs_backward takes the forward's d_stats */
+
+/* Log probabilities of given tokens, entropy and top alternatives.  Row i, with m = max_j z_ij and S = sum_j exp(z_ij - m):
+ *   log p_ij = (z_ij - m) - log S      H_i = -sum_j p_ij log p_ij
+ *  d_logits     : [n_rows, n_classes], rows row_stride apart
+ *  d_tokens     : DC_TOKENS_*[n_rows] or NULL (then d_logprob is not written and no row is skipped)
+ *  ignore_token : a row whose token is this one (labels: DC_IGNORE_LABEL on padding) is SKIPPED: its logits are not read,
+ *                 its outputs are 0 and its alternatives -1.  A token outside [0, n_classes) otherwise: log probability NaN.
+ *  d_logprob    : float[n_rows], d_entropy: float[n_rows]; either or NULL
+ *  d_stats      : float[n_rows, 3] = m, log S, H for the backward pass, or NULL
+ *  d_top_ids, d_top_logprob: int32 / float[n_rows, n_top]: the n_top (<= n_classes, <= DC_MAX_TOP) classes of the largest
+ *                 logits in descending order, ties to the lower class, and their log probabilities; n_top = 0: NULL.
+ *  Logits of -inf are classes that cannot be: probability 0.  A row of nothing else has log probabilities -inf, entropy 0 and
+ *  zero gradients.  A NaN or +inf in a row makes its log probabilities and entropy NaN (NaN sorts as the largest). */
+int dc_token_logprobs(void* stream, const void* d_logits, int32_t dtype, int64_t n_rows, int32_t n_classes,
+                      int64_t row_stride, const void* d_tokens, int32_t token_type, int64_t ignore_token, int32_t n_top,
+                      float* d_logprob, float* d_entropy, float* d_stats, int32_t* d_top_ids, float* d_top_logprob,
+                      void* d_workspace, int64_t workspace_bytes);
+int64_t dc_token_logprobs_workspace(int64_t n_rows, int32_t n_classes, int32_t n_top);
+
+/* Gradient of the two: d_grad_logits[i,j] = p_ij (-g_i - h_i (log p_ij + H_i)) + g_i [j = token_i] with g = d_grad_logprob,
+ * h = d_grad_entropy (either may be NULL: zero).  Skipped rows get zeros, rows with a token outside the classes NaN.
+ *  d_tokens : or NULL when d_grad_logprob is;  d_stats: of the forward call; NULL is fine for n_classes < DC_STATS_FROM,
+ *             where the row is still in registers and re-deriving costs less than reading it
+ *  d_grad_logits: the logits' type, rows grad_stride apart; it may be d_logits itself */
+int dc_token_logprobs_backward(void* stream, const void* d_logits, int32_t dtype, int64_t n_rows, int32_t n_classes,
+                               int64_t row_stride, const void* d_tokens, int32_t token_type, int64_t ignore_token,
+                               const float* d_stats, const float* d_grad_logprob, const float* d_grad_entropy,
+                               void* d_grad_logits, int64_t grad_stride);
+
+/* Gated linear recurrence over every channel of every sequence:
+ *   a_t = sigmoid(f_t)    h_t = a_t h_(t-1) + (1 - a_t) x_t    y_t = h_t,   t along the sequence, or from its end (reverse)
+ *  d_x, d_f   : [n_tokens, n_channels]; a gate of +inf keeps the state whatever x holds, -inf takes x whatever the state holds
+ *  d_begin, d_end: int64[n_seqs] on the device, sequence s = tokens [begin[s], end[s]) (offsets of a packed batch: pass
+ *               offsets and offsets + 1), which may not overlap, or both NULL: n_seqs dense sequences of max_len tokens
+ *  max_len    : no sequence is longer (host value: it shapes the launch)
+ *  d_h0       : float[n_seqs, n_channels] state before the first token, or NULL (zeros)
+ *  d_y        : [n_tokens, n_channels], not overlapping the inputs; tokens of no sequence are left untouched, or with
+ *               zero_rest != 0 those in front of begin[0] and from end[n_seqs - 1] on (all, where there is no sequence) set to 0
+ *  d_h_last   : float[n_seqs, n_channels] state after the last token, or NULL; it may be d_h0 (a state kept in place)
+ *  d_saved    : dc_gated_scan_saved(...) floats for the backward pass, or NULL
+ *  A sequence with begin < 0, end < begin, end > n_tokens or more than max_len tokens is refused on the device: its d_h_last
+ *  row (backward: d_grad_h0 row) is NaN and nothing else of it is written. */
+int dc_gated_scan(void* stream, int32_t dtype, const void* d_x, int64_t x_stride, const void* d_f, int64_t f_stride,
+                  int64_t n_tokens, int32_t n_channels, const int64_t* d_begin, const int64_t* d_end, int32_t n_seqs,
+                  int64_t max_len, int32_t reverse, const float* d_h0, void* d_y, int64_t y_stride, int32_t zero_rest,
+                  float* d_h_last, float* d_saved, void* d_workspace, int64_t workspace_bytes);
+int64_t dc_gated_scan_workspace(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max_len);
+/* floats of d_saved: the state on entering every 128-token tile of [0, n_tokens) */
+int64_t dc_gated_scan_saved(int64_t n_tokens, int32_t n_channels);
+
+/* Its backward pass.  With g_t = dy_t + a_(t+1) g_(t+1), plus d_grad_h_last at the last token:
+ *   dx_t = (1 - a_t) g_t    df_t = g_t (h_(t-1) - x_t) a_t (1 - a_t)    dh0 = a_0 g_0
+ *  inputs as in the forward call, d_saved as it left it; d_grad_h_last or NULL; d_grad_h0 or NULL.
+ *  The states between two tiles are computed again from d_saved in fp32 (y, rounded, is not read).
+ *  d_grad_x, d_grad_f: [n_tokens, n_channels]; tokens of no sequence as in d_y. */
+int dc_gated_scan_backward(void* stream, int32_t dtype, const void* d_x, int64_t x_stride, const void* d_f, int64_t f_stride,
+                           int64_t n_tokens, int32_t n_channels, const int64_t* d_begin, const int64_t* d_end,
+                           int32_t n_seqs, int64_t max_len, int32_t reverse, const float* d_h0, const float* d_saved,
+                           const void* d_grad_y, int64_t grad_y_stride, const float* d_grad_h_last, void* d_grad_x,
+                           int64_t grad_x_stride, void* d_grad_f, int64_t grad_f_stride, int32_t zero_rest,
+                           float* d_grad_h0, void* d_workspace, int64_t workspace_bytes);
+
+/* What stands between two blocks: the norm behind one, its gate and residual scale, and the norm in front of the next.
+ *   u = norm(y) * post_w + post_b  (post_norm = 0: u = y)     v = act(gate) * u  (d_gate NULL: v = u)
+ *   r' = residual + scale * v                                 n = norm(r') * pre_w + pre_b
+ *   norm(x) = (x - mean) / sqrt(var + eps) (DC_NORM_LAYER) or x / sqrt(mean(x^2) + eps) (DC_NORM_RMS)
+ *  dtype          : of y, gate and n;  residual_dtype: of residual and r', DC_DTYPE_F32 or dtype.  n is taken of r' in fp32,
+ *                   before r' is rounded
+ *  d_y            : NULL: no block in front (r' = residual; the first norm of a model);  d_residual NULL: r' = scale * v
+ *  d_scale, d_*_w : float[width] or NULL (ones);  d_*_b: float[width] or NULL (zeros)
+ *  d_residual_out : or NULL (not stored); it may be d_residual itself;  d_normed: or NULL (no norm in front of a next block) */
+int dc_block_norm(void* stream, int32_t dtype, int32_t residual_dtype, int64_t n_rows, int32_t width, int32_t kind,
+                  float eps, const void* d_y, int64_t y_stride, const void* d_gate, int64_t gate_stride, int32_t gate_act,
+                  const void* d_residual, int64_t residual_stride, const float* d_scale, int32_t post_norm,
+                  const float* d_post_w, const float* d_post_b, const float* d_pre_w, const float* d_pre_b,
+                  void* d_residual_out, int64_t residual_out_stride, void* d_normed, int64_t normed_stride);
+
+/* Its backward pass: the same inputs (d_residual as it was BEFORE the forward call), and the gradients of r' and n
+ * (either or NULL: zero).  r', the norms' statistics and u are computed again from the inputs.
+ *  d_grad_y, d_grad_gate, d_grad_residual: dense, or NULL;  d_grad_scale, d_grad_*_w, d_grad_*_b: float[width], or NULL
+ *  (summed over the rows in a fixed order). */
+int dc_block_norm_backward(void* stream, int32_t dtype, int32_t residual_dtype, int64_t n_rows, int32_t width, int32_t kind,
+                           float eps, const void* d_y, int64_t y_stride, const void* d_gate, int64_t gate_stride,
+                           int32_t gate_act, const void* d_residual, int64_t residual_stride, const float* d_scale,
+                           int32_t post_norm, const float* d_post_w, const float* d_post_b, const float* d_pre_w,
+                           const void* d_grad_residual_out, int64_t grad_residual_out_stride, const void* d_grad_normed,
+                           int64_t grad_normed_stride, void* d_grad_y, void* d_grad_gate, void* d_grad_residual,
+                           float* d_grad_scale, float* d_grad_post_w, float* d_grad_post_b, float* d_grad_pre_w,
+                           float* d_grad_pre_b, void* d_workspace, int64_t workspace_bytes);
+int64_t dc_block_norm_workspace(int64_t n_rows, int32_t width);
+
 #ifdef __cplusplus
 }
 #endif
