@@ -1,105 +1,88 @@
 // dc_gated_scan: h_t = a_t h_(t-1) + (1 - a_t) x_t with a = sigmoid(f), per channel of every sequence, and its backward pass.
 //
-// A gate has two weights, a and 1 - a, and fp32 holds only the smaller of them to full relative accuracy:
-// p = min(a, 1 - a) = e / (1 + e), e = exp(-|f|).  Each step is written as a move by p from the one operand towards the other,
-//   f > 0: h' = h + p (x - h)        f <= 0: h' = x + p (h - x)
-// so a gate that keeps 99.99 % for thousands of tokens loses no more than one that forgets at once (a * h + (1 - a) * x with
-// a rounded to 1 - 2^-24 steps drifts by 2^-25 / (1 - a)).  p = 0 selects its operand: a gate of +-inf never touches the other.
+// Arithmetic.  A gate has two weights, a and 1 - a, and fp32 holds only the smaller of them to full relative accuracy:
+// p = min(a, 1 - a) = e / (1 + e), e = exp(-|f|).  Each step is a move by p from one operand towards the other,
+//   f > 0: h' = h + p (x - h)        f <= 0: h' = x - p (x - h)
+// so a gate that keeps 99.99 % for thousands of tokens loses no more than one that forgets at once (with a rounded, a h would
+// drift by 2^-25 a step).  A span of steps is the map h -> H + A h; it carries both A and G = 1 - A and is applied with the
+// smaller of them, for the same reason.  Weights below 2^-126 are 0.
+//
+// Form.  HBM-bound: 3 elements of traffic per element forward, 5 backward, about 30 and 50 vector operations.  Lanes run along the
+// channels (a row of 64 lanes is 256 contiguous bytes), time is divided: a workgroup's 8 wavefronts take 8 consecutive tokens each of
+// a 64-token tile (narrow batches: 16 or 32 lanes a row and 32 or 16 such groups), keep them in registers, pass each other their
+// maps through LDS and run the steps again from the state they then know.  Where sequences and channels alone do not fill the chip,
+// a sequence is divided into chunks: a first kernel reads each chunk for its map alone, the second starts from the composed maps.
+#include <initializer_list>
+#include <type_traits>
+
 #include "elem_io.h"
 
 namespace dc {
 namespace {
 
-constexpr int kTile = 128;  // tokens between two states of d_saved
+constexpr int kTile = 64;      // tokens between two states of d_saved
+constexpr int kThreads = 512;  // a workgroup
+constexpr int kSteps = 8;      // consecutive tokens of one group of lanes: their inputs live in registers
+constexpr int kShort = 16;     // sequences up to here: a thread per channel, token after token
+constexpr int kZeroBlocks = 32;
 
 struct ScanArgs {
   const int64_t* begin;  // or null: dense sequences of max_len tokens
   const int64_t* end;
   int64_t n_tokens, max_len;
   int32_t n_seqs, n_channels, reverse;
+  int32_t lane_bits;  // log2 of the lanes along the channels
+  int32_t n_chunks;   // chunks of a sequence ...
+  int64_t chunk;      // ... of so many tokens each (a multiple of the workgroup's tile)
+  int32_t n_blocks;   // workgroups of the recurrence; those behind them write the zeros of zero_rest
 };
 
-// [b, e) of sequence s; false: the sequence breaks the contract
-__device__ __forceinline__ bool seq_range(const ScanArgs& a, int s, int64_t* b, int64_t* e) {
-  *b = a.begin ? a.begin[s] : s * a.max_len;
-  *e = a.end ? a.end[s] : *b + a.max_len;
-  return *b >= 0 && *e >= *b && *e <= a.n_tokens && *e - *b <= a.max_len;
-}
-
-__device__ __forceinline__ float step(float h, float x, float f) {
-  const float p = gate_minor(f);
-  const float base = f > 0.0f ? h : x, other = f > 0.0f ? x : h;
-  return p == 0.0f ? base : __builtin_fmaf(p, other - base, base);
-}
-
-// A thread per channel of a sequence.
-template <typename T>
-__global__ __launch_bounds__(64) void scan_walk_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f, int64_t ldf,
-                                                       const float* h0, T* __restrict__ y, int64_t ldy, float* h_last,
-                                                       float* __restrict__ saved) {
-  const int blocks = (a.n_channels + 63) / 64;
-  const int s = blockIdx.x / blocks, c = blockIdx.x % blocks * 64 + threadIdx.x;
-  if (c >= a.n_channels) return;
-  int64_t b, e;
-  const bool ok = seq_range(a, s, &b, &e);
-  float h = h0 ? h0[(int64_t)s * a.n_channels + c] : 0.0f;
-  if (ok) {
-    for (int64_t i = 0; i < e - b; ++i) {
-      const int64_t t = a.reverse ? e - 1 - i : b + i;
-      if (saved && (a.reverse ? t % kTile == kTile - 1 : t % kTile == 0)) saved[t / kTile * a.n_channels + c] = h;
-      h = step(h, (float)x[t * ldx + c], (float)f[t * ldf + c]);
-      y[t * ldy + c] = (T)h;
-    }
+// A sequence in the order of the recurrence: its token j is row base + dir * j.
+struct Seq {
+  int64_t base, len;
+  int32_t dir;
+  bool ok;
+  __device__ __forceinline__ Seq(const ScanArgs& a, int s) {
+    const int64_t b = a.begin ? a.begin[s] : s * a.max_len, e = a.end ? a.end[s] : b + a.max_len;
+    ok = b >= 0 && e >= b && e <= a.n_tokens && e - b <= a.max_len;
+    len = ok ? e - b : 0;
+    base = a.reverse ? e - 1 : b;
+    dir = a.reverse ? -1 : 1;
   }
-  if (h_last) h_last[(int64_t)s * a.n_channels + c] = ok ? h : __builtin_nanf("");
+  __device__ __forceinline__ int64_t row(int64_t j) const { return dir < 0 ? base - j : base + j; }
+};
+
+// The gate's smaller weight, with the gate's sign: non-negative where the state is what is moved, negative where x is.
+__device__ __forceinline__ float signed_gate(float f) { return __builtin_copysignf(gate_minor(f), f); }
+__device__ __forceinline__ bool keeps(float ps) { return __float_as_int(ps) >= 0; }
+__device__ __forceinline__ float step(float h, float x, float ps) { return __builtin_fmaf(ps, x - h, keeps(ps) ? h : x); }
+// a * v
+__device__ __forceinline__ float decay(float v, float ps) { return keeps(ps) ? __builtin_fmaf(-ps, v, v) : -ps * v; }
+
+// x where it counts: a gate of +inf (or one whose other weight is 0 in fp32) does not look at it
+__device__ __forceinline__ float seen(float x, float ps) { return __float_as_int(ps) == 0 ? 0.0f : x; }
+
+// A span of steps: h -> H + A h, G = 1 - A
+struct Span {
+  float A, G, H;
+};
+__device__ __forceinline__ Span identity_span() { return {1.0f, 0.0f, 0.0f}; }
+__device__ __forceinline__ float apply(float A, float G, float H, float h) {
+  return A > 0.5f ? h + __builtin_fmaf(-G, h, H) : __builtin_fmaf(A, h, H);
+}
+__device__ __forceinline__ void extend(float& A, float& G, float ps) {  // by one step
+  const float p = __builtin_fabsf(ps), q = 1.0f - p;
+  const bool k = keeps(ps);
+  A *= k ? q : p;
+  G = __builtin_fmaf(k ? p : q, 1.0f - G, G);
+}
+__device__ __forceinline__ Span then(const Span& a, const Span& b) {  // a, then b
+  return {a.A * b.A, __builtin_fmaf(b.G, 1.0f - a.G, a.G), apply(b.A, b.G, b.H, a.H)};
 }
 
-// A thread per channel of a sequence, tile by tile from its last token on: the states of a tile again from the one it was
-// entered with, kept in LDS, then the gradients against the direction of the recurrence.
+// the rows in front of the first and behind the last sequence, to zero
 template <typename T>
-__global__ __launch_bounds__(64) void scan_walk_backward_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f, int64_t ldf,
-                                                                const float* __restrict__ h0, const float* __restrict__ saved,
-                                                                const T* __restrict__ gy, int64_t ldgy, const float* g_last,
-                                                                T* __restrict__ gx, int64_t ldgx, T* __restrict__ gf, int64_t ldgf, float* g_h0) {
-  __shared__ float before[kTile][64];
-  const int blocks = (a.n_channels + 63) / 64;
-  const int s = blockIdx.x / blocks, c = blockIdx.x % blocks * 64 + threadIdx.x;
-  if (c >= a.n_channels) return;
-  int64_t b, e;
-  const bool ok = seq_range(a, s, &b, &e);
-  const int64_t sc = (int64_t)s * a.n_channels + c;
-  float g = g_last ? g_last[sc] : 0.0f;
-  if (ok) {
-    for (int64_t left = e - b; left > 0;) {  // tokens i = 0 .. left - 1 (in the recurrence's order) are still to do
-      const int64_t last = a.reverse ? e - left : b + left - 1;
-      const int64_t tile = last / kTile;
-      const int64_t in_tile = a.reverse ? (tile + 1) * kTile - last : last - tile * kTile + 1;
-      const int n = (int)(in_tile < left ? in_tile : left);
-      float h = in_tile <= left ? saved[tile * a.n_channels + c] : h0 ? h0[sc] : 0.0f;
-      for (int k = 0; k < n; ++k) {
-        const int64_t i = left - n + k, t = a.reverse ? e - 1 - i : b + i;
-        before[k][threadIdx.x] = h;
-        h = step(h, (float)x[t * ldx + c], (float)f[t * ldf + c]);
-      }
-      for (int k = n - 1; k >= 0; --k) {
-        const int64_t i = left - n + k, t = a.reverse ? e - 1 - i : b + i;
-        const float xt = (float)x[t * ldx + c], ft = (float)f[t * ldf + c];
-        const float p = gate_minor(ft);
-        g += (float)gy[t * ldgy + c];
-        const float pg = p == 0.0f ? 0.0f : p * g, rest = g - pg;
-        gx[t * ldgx + c] = (T)(ft > 0.0f ? pg : rest);
-        gf[t * ldgf + c] = (T)(p == 0.0f ? 0.0f : pg * (1.0f - p) * (before[k][threadIdx.x] - xt));
-        g = ft > 0.0f ? rest : pg;
-      }
-      left -= n;
-    }
-  }
-  if (g_h0) g_h0[sc] = ok ? g : __builtin_nanf("");
-}
-
-// zeros in the tokens in front of the first and behind the last sequence (rows blockIdx.x, blockIdx.x + gridDim.x, ... of them)
-template <typename T>
-__global__ __launch_bounds__(256) void zero_rest_kernel(ScanArgs a, T* y, int64_t ldy, T* y2, int64_t ldy2) {
+__device__ void zero_rest(const ScanArgs& a, int block, T* y, int64_t ldy, T* y2, int64_t ldy2) {
   int64_t b = a.n_tokens, e = a.n_tokens;
   if (a.n_seqs > 0) {
     b = a.begin ? a.begin[0] : 0;
@@ -107,7 +90,7 @@ __global__ __launch_bounds__(256) void zero_rest_kernel(ScanArgs a, T* y, int64_
     b = b < 0 ? 0 : b > a.n_tokens ? a.n_tokens : b;
     e = e < b ? b : e > a.n_tokens ? a.n_tokens : e;
   }
-  for (int64_t i = blockIdx.x; i < b + a.n_tokens - e; i += gridDim.x) {
+  for (int64_t i = block; i < b + a.n_tokens - e; i += kZeroBlocks) {
     const int64_t t = i < b ? i : i - b + e;
     for (int c = threadIdx.x; c < a.n_channels; c += blockDim.x) {
       y[t * ldy + c] = (T)0.0f;
@@ -116,16 +99,490 @@ __global__ __launch_bounds__(256) void zero_rest_kernel(ScanArgs a, T* y, int64_
   }
 }
 
+// ---- sequences of at most kShort tokens: a thread per V channels ---------------------------------------------------------------
+constexpr int kWalkThreads = 64;
+
+template <typename T, int V>
+__global__ __launch_bounds__(kWalkThreads) void scan_walk_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f, int64_t ldf,
+                                                                 const float* h0, T* __restrict__ y, int64_t ldy, float* h_last) {
+  if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, y, ldy, nullptr, 0);
+  const int per_seq = (a.n_channels + kWalkThreads * V - 1) / (kWalkThreads * V);
+  const int s = blockIdx.x / per_seq, c = (blockIdx.x % per_seq * kWalkThreads + threadIdx.x) * V;
+  if (c >= a.n_channels) return;
+  const Seq q(a, s);
+  const int64_t sc = (int64_t)s * a.n_channels + c;
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = h0 ? h0[sc + v] : 0.0f;
+#pragma unroll 4
+  for (int64_t j = 0; j < q.len; ++j) {
+    const int64_t t = q.row(j);
+    float xv[V], fv[V];
+    load_vec<V>(x + t * ldx + c, xv);
+    load_vec<V>(f + t * ldf + c, fv);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float ps = signed_gate(fv[v]);
+      h[v] = step(h[v], seen(xv[v], ps), ps);
+    }
+    store_vec<V>(y + t * ldy + c, h);
+  }
+  if (h_last) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) h_last[sc + v] = q.ok ? h[v] : __builtin_nanf("");
+  }
+}
+
+// The states again from h0, kept in LDS, then the gradients from the last token back.
+template <typename T, int V>
+__global__ __launch_bounds__(kWalkThreads) void scan_walk_backward_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f, int64_t ldf,
+                                                                          const float* __restrict__ h0, const T* __restrict__ gy, int64_t ldgy,
+                                                                          const float* g_last, T* __restrict__ gx, int64_t ldgx, T* __restrict__ gf,
+                                                                          int64_t ldgf, float* g_h0) {
+  if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, gx, ldgx, gf, ldgf);
+  __shared__ float above[kShort][kWalkThreads * V];  // h_(t-1) - x_t
+  const int per_seq = (a.n_channels + kWalkThreads * V - 1) / (kWalkThreads * V);
+  const int s = blockIdx.x / per_seq, c = (blockIdx.x % per_seq * kWalkThreads + threadIdx.x) * V;
+  if (c >= a.n_channels) return;
+  const Seq q(a, s);
+  const int64_t sc = (int64_t)s * a.n_channels + c;
+  const int n = (int)q.len;
+  float h[V], g[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = h0 ? h0[sc + v] : 0.0f, g[v] = g_last ? g_last[sc + v] : 0.0f;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const int64_t t = q.row(j);
+    float xv[V], fv[V];
+    load_vec<V>(x + t * ldx + c, xv);
+    load_vec<V>(f + t * ldf + c, fv);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float ps = signed_gate(fv[v]), xs = seen(xv[v], ps);
+      above[j][threadIdx.x * V + v] = h[v] - xs;
+      h[v] = step(h[v], xs, ps);
+    }
+  }
+#pragma unroll 4
+  for (int j = n - 1; j >= 0; --j) {
+    const int64_t t = q.row(j);
+    float fv[V], yv[V], ox[V], of[V];
+    load_vec<V>(f + t * ldf + c, fv);
+    load_vec<V>(gy + t * ldgy + c, yv);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float ps = signed_gate(fv[v]), p = __builtin_fabsf(ps);
+      const float total = g[v] + yv[v];
+      g[v] = decay(total, ps);
+      ox[v] = keeps(ps) ? p * total : __builtin_fmaf(ps, total, total);
+      of[v] = p * (1.0f - p) * total * above[j][threadIdx.x * V + v];
+    }
+    store_vec<V>(gx + t * ldgx + c, ox);
+    store_vec<V>(gf + t * ldgf + c, of);
+  }
+  if (g_h0) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) g_h0[sc + v] = q.ok ? g[v] : __builtin_nanf("");
+  }
+}
+
+// ---- longer sequences: tiles of (kThreads >> lane_bits) groups of kSteps tokens --------------------------------------------------
+// Which sequence, chunk, channels and group of tokens a thread works on.
+template <int V>
+struct Place {
+  int s, chunk, group, n_groups, channel, slot;  // slot: of this thread's channels in a group's row of LDS
+  bool active;
+  __device__ __forceinline__ Place(const ScanArgs& a) {
+    const int lanes = 1 << a.lane_bits, per_row = (a.n_channels + lanes * V - 1) / (lanes * V);
+    const int lane = threadIdx.x & (lanes - 1);
+    group = threadIdx.x >> a.lane_bits;
+    n_groups = kThreads >> a.lane_bits;
+    channel = ((int)blockIdx.x % per_row * lanes + lane) * V;
+    chunk = (int)blockIdx.x / per_row % a.n_chunks;
+    s = (int)blockIdx.x / per_row / a.n_chunks;
+    slot = lane * V;
+    active = channel < a.n_channels;
+  }
+  __device__ __forceinline__ int at(int grp, int lanes_v) const { return grp * lanes_v + slot; }
+};
+
+// kSteps rows of V channels, raw; rows from n on are not read
+template <typename T, int V>
+struct Rows {
+  vec_t<T, V> r[kSteps];
+  __device__ __forceinline__ void load(const T* p, int64_t ld, int n) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      if (i < n) {
+        if constexpr (V == 1) r[i][0] = p[i * ld];
+        else r[i] = *reinterpret_cast<const vec_t<T, V>*>(p + i * ld);
+      } else {
+        r[i] = vec_t<T, V>(0);
+      }
+    }
+  }
+};
+
+// Chunk maps in the workspace: [sequence][chunk][A, G, H][channel], and behind them the states the sequences start from.
+__device__ __forceinline__ int64_t map_at(const ScanArgs& a, int s, int chunk, int k, int channel) {
+  return (((int64_t)s * a.n_chunks + chunk) * 3 + k) * a.n_channels + channel;
+}
+__device__ __forceinline__ int64_t start_at(const ScanArgs& a, int s, int channel) {
+  return ((int64_t)a.n_seqs * a.n_chunks * 3 + s) * a.n_channels + channel;
+}
+
+// The map of every chunk, forward (x is the third input) or backward (c -> Q + A c against the recurrence; gy is).  Every group of lanes
+// walks its own part of the chunk; one exchange at the end.  `start` (h0 or the gradient of h_last, or null) is copied behind the maps:
+// the second kernel may then write where it came from.
+template <typename T, int V, bool BACK>
+__global__ __launch_bounds__(kThreads) void scan_map_kernel(ScanArgs a, const T* __restrict__ f, int64_t ldf, const T* __restrict__ x, int64_t ldx,
+                                                            const float* start, float* __restrict__ maps) {
+  __shared__ float lds[3][kThreads * V];
+  const Place<V> at(a);
+  const Seq q(a, at.s);
+  const int lanes_v = V << a.lane_bits;
+  const int64_t j0 = at.chunk * a.chunk, part = a.chunk / at.n_groups;
+  if (at.chunk == 0 && at.active && at.group == 0) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      maps[start_at(a, at.s, at.channel + v)] = start ? start[(int64_t)at.s * a.n_channels + at.channel + v] : 0.0f;
+  }
+  if (j0 >= q.len) return;
+  const int64_t p0 = j0 + at.group * part, p1 = p0 + part < q.len ? p0 + part : q.len;
+  Span m[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) m[v] = identity_span();
+  if (at.active) {
+    const int64_t sf = q.dir * ldf, sx = q.dir * ldx;
+    const int n_blocks = p1 > p0 ? (int)((p1 - p0 + kSteps - 1) / kSteps) : 0;
+    for (int b = 0; b < n_blocks; ++b) {
+      const int64_t j = p0 + (int64_t)(BACK ? n_blocks - 1 - b : b) * kSteps;
+      const int n = p1 - j < kSteps ? (int)(p1 - j) : kSteps;
+      Rows<T, V> rf, rx;
+      rf.load(f + q.row(j) * ldf + at.channel, sf, n);
+      rx.load(x + q.row(j) * ldx + at.channel, sx, n);
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const int i = BACK ? kSteps - 1 - k : k;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float ps = i < n ? signed_gate((float)rf.r[i][v]) : 0.0f, xv = (float)rx.r[i][v];
+          extend(m[v].A, m[v].G, ps);
+          m[v].H = BACK ? decay(m[v].H + xv, ps) : step(m[v].H, seen(xv, ps), ps);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = at.at(at.group, lanes_v) + v;
+    lds[0][i] = m[v].A, lds[1][i] = m[v].G, lds[2][i] = m[v].H;
+  }
+  __syncthreads();
+  if (at.group != 0 || !at.active) return;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    Span all = identity_span();
+    for (int k = 0; k < at.n_groups; ++k) {
+      const int i = at.at(BACK ? at.n_groups - 1 - k : k, lanes_v) + v;
+      all = then(all, Span{lds[0][i], lds[1][i], lds[2][i]});
+    }
+    maps[map_at(a, at.s, at.chunk, 0, at.channel + v)] = all.A;
+    maps[map_at(a, at.s, at.chunk, 1, at.channel + v)] = all.G;
+    maps[map_at(a, at.s, at.chunk, 2, at.channel + v)] = all.H;
+  }
+}
+
+// What a chunk starts from: the sequence's start through the maps of chunks [from, from + n) (dir 1) or (from, from - n] downwards
+// (dir -1); the groups of lanes compose a part each.  Ends with a barrier behind the last use of `lds`.
+template <int V>
+__device__ void compose_chunks(const ScanArgs& a, const Place<V>& at, const float* __restrict__ maps, int from, int dir, int n, float (*lds)[kThreads * V],
+                               float (&h)[V]) {
+  const int lanes_v = V << a.lane_bits;
+  Span m[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) m[v] = identity_span();
+  if (at.active) {
+    const int lo = (int)((int64_t)n * at.group / at.n_groups), hi = (int)((int64_t)n * (at.group + 1) / at.n_groups);
+#pragma unroll 4
+    for (int k = lo; k < hi; ++k) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int64_t i = map_at(a, at.s, from + dir * k, 0, at.channel + v);
+        m[v] = then(m[v], Span{maps[i], maps[i + a.n_channels], maps[i + 2 * (int64_t)a.n_channels]});
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = at.at(at.group, lanes_v) + v;
+    lds[0][i] = m[v].A, lds[1][i] = m[v].G, lds[2][i] = m[v].H;
+    h[v] = at.active ? maps[start_at(a, at.s, at.channel + v)] : 0.0f;
+  }
+  __syncthreads();
+  for (int k = 0; k < at.n_groups; ++k) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = at.at(k, lanes_v) + v;
+      h[v] = apply(lds[0][i], lds[1][i], lds[2][i], h[v]);
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads, 2) void scan_tile_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f, int64_t ldf,
+                                                                const float* h0, T* __restrict__ y, int64_t ldy, float* h_last,
+                                                                float* __restrict__ saved, const float* __restrict__ maps) {
+  __shared__ float lds[2][3][kThreads * V];
+  if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, y, ldy, nullptr, 0);
+  const Place<V> at(a);
+  const Seq q(a, at.s);
+  const int lanes_v = V << a.lane_bits, tile = at.n_groups * kSteps;
+  const int64_t sc = (int64_t)at.s * a.n_channels + at.channel;
+  const int64_t j0 = at.chunk * a.chunk, j1 = j0 + a.chunk < q.len ? j0 + a.chunk : q.len;
+  if (j0 >= q.len && at.chunk > 0) return;
+  float carry[V];
+  if (maps) {
+    compose_chunks<V>(a, at, maps, 0, 1, at.chunk, lds[0], carry);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = h0 && at.active ? h0[sc + v] : 0.0f;
+  }
+  const int64_t sx = q.dir * ldx, sf = q.dir * ldf, sy = q.dir * ldy;
+  int turn = 0;
+  for (int64_t jt = j0; jt < j1; jt += tile, turn ^= 1) {
+    const int64_t j = jt + at.group * kSteps, left = j1 - j;
+    const int n = !at.active || left <= 0 ? 0 : left < kSteps ? (int)left : kSteps;
+    Rows<T, V> rx, rf;
+    rx.load(x + q.row(j) * ldx + at.channel, sx, n);
+    rf.load(f + q.row(j) * ldf + at.channel, sf, n);
+    float xs[kSteps][V], ps[kSteps][V];
+    Span m[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) m[v] = identity_span();
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        ps[i][v] = i < n ? signed_gate((float)rf.r[i][v]) : 0.0f;
+        xs[i][v] = seen((float)rx.r[i][v], ps[i][v]);
+        extend(m[v].A, m[v].G, ps[i][v]);
+        m[v].H = step(m[v].H, xs[i][v], ps[i][v]);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = at.at(at.group, lanes_v) + v;
+      lds[turn][0][i] = m[v].A, lds[turn][1][i] = m[v].G, lds[turn][2][i] = m[v].H;
+    }
+    __syncthreads();  // (one a tile: the next tile writes the other half)
+    float h[V];
+    for (int k = 0; k < at.n_groups; ++k) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int i = at.at(k, lanes_v) + v;
+        if (k == at.group) h[v] = carry[v];
+        carry[v] = apply(lds[turn][0][i], lds[turn][1][i], lds[turn][2][i], carry[v]);
+      }
+    }
+    if (n > 0) {
+      if (saved && j % kTile == 0 && j > 0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) saved[q.row(j) / kTile * a.n_channels + at.channel + v] = h[v];
+      }
+      T* out = y + q.row(j) * ldy + at.channel;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = step(h[v], xs[i][v], ps[i][v]);
+        if (i < n) store_vec<V>(out + i * sy, h);
+      }
+    }
+  }
+  if (h_last && at.group == 0 && at.active && j1 == q.len) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) h_last[sc + v] = q.ok ? carry[v] : __builtin_nanf("");
+  }
+}
+
+// Tiles from the last one back.  The state a tile was entered with comes from `saved`; maps of the states and of what comes back go
+// through the same exchange.
+template <typename T, int V>
+__global__ __launch_bounds__(kThreads, 2) void scan_tile_backward_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f,
+                                                                         int64_t ldf, const float* __restrict__ h0, const float* __restrict__ saved,
+                                                                         const T* __restrict__ gy, int64_t ldgy, const float* g_last,
+                                                                         T* __restrict__ gx, int64_t ldgx, T* __restrict__ gf, int64_t ldgf, float* g_h0,
+                                                                         const float* __restrict__ maps) {
+  __shared__ float lds[2][4][kThreads * V];
+  if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, gx, ldgx, gf, ldgf);
+  const Place<V> at(a);
+  const Seq q(a, at.s);
+  const int lanes_v = V << a.lane_bits, tile = at.n_groups * kSteps;
+  const int64_t sc = (int64_t)at.s * a.n_channels + at.channel;
+  const int64_t j0 = at.chunk * a.chunk, j1 = j0 + a.chunk < q.len ? j0 + a.chunk : q.len;
+  if (j0 >= q.len && at.chunk > 0) return;
+  float carry[V];  // a_t g_t of the token behind
+  if (maps) {
+    const int last = q.len > 0 ? (int)((q.len - 1) / a.chunk) : 0;
+    compose_chunks<V>(a, at, maps, last, -1, last - at.chunk, lds[0], carry);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = g_last && at.active ? g_last[sc + v] : 0.0f;
+  }
+  const int64_t sx = q.dir * ldx, sf = q.dir * ldf, sy = q.dir * ldgy;
+  int turn = 0;
+  const int64_t tiles = j1 > j0 ? (j1 - j0 + tile - 1) / tile : 0;
+  for (int64_t k = tiles - 1; k >= 0; --k, turn ^= 1) {
+    const int64_t jt = j0 + k * tile, j = jt + at.group * kSteps, left = j1 - j;
+    const int n = !at.active || left <= 0 ? 0 : left < kSteps ? (int)left : kSteps;
+    Rows<T, V> rx, rf, ry;
+    rx.load(x + q.row(j) * ldx + at.channel, sx, n);
+    rf.load(f + q.row(j) * ldf + at.channel, sf, n);
+    ry.load(gy + q.row(j) * ldgy + at.channel, sy, n);
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      h[v] = !at.active ? 0.0f : jt > 0 ? saved[q.row(jt) / kTile * a.n_channels + at.channel + v] : h0 ? h0[sc + v] : 0.0f;
+    float xs[kSteps][V], ps[kSteps][V], Q[V];
+    Span m[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) m[v] = identity_span(), Q[v] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        ps[i][v] = i < n ? signed_gate((float)rf.r[i][v]) : 0.0f;
+        xs[i][v] = seen((float)rx.r[i][v], ps[i][v]);
+        extend(m[v].A, m[v].G, ps[i][v]);
+        m[v].H = step(m[v].H, xs[i][v], ps[i][v]);
+      }
+    }
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) Q[v] = decay(Q[v] + (float)ry.r[i][v], ps[i][v]);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = at.at(at.group, lanes_v) + v;
+      lds[turn][0][i] = m[v].A, lds[turn][1][i] = m[v].G, lds[turn][2][i] = m[v].H, lds[turn][3][i] = Q[v];
+    }
+    __syncthreads();
+    float c[V];
+    for (int b = 0; b < at.n_groups; ++b) {
+      const int back = at.n_groups - 1 - b;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int i = at.at(b, lanes_v) + v, o = at.at(back, lanes_v) + v;
+        if (b < at.group) h[v] = apply(lds[turn][0][i], lds[turn][1][i], lds[turn][2][i], h[v]);
+        if (back == at.group) c[v] = carry[v];
+        carry[v] = apply(lds[turn][0][o], lds[turn][1][o], lds[turn][3][o], carry[v]);
+      }
+    }
+    if (n > 0) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float above = h[v] - xs[i][v];
+          h[v] = step(h[v], xs[i][v], ps[i][v]);
+          xs[i][v] = above;
+        }
+      }
+      T *ox = gx + q.row(j) * ldgx + at.channel, *of = gf + q.row(j) * ldgf + at.channel;
+#pragma unroll
+      for (int i = kSteps - 1; i >= 0; --i) {
+        float dx[V], df[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float p = __builtin_fabsf(ps[i][v]), total = c[v] + (float)ry.r[i][v];
+          c[v] = decay(total, ps[i][v]);
+          dx[v] = keeps(ps[i][v]) ? p * total : __builtin_fmaf(ps[i][v], total, total);
+          df[v] = p * (1.0f - p) * total * xs[i][v];
+        }
+        if (i < n) {
+          store_vec<V>(ox + i * (q.dir * ldgx), dx);
+          store_vec<V>(of + i * (q.dir * ldgf), df);
+        }
+      }
+    }
+  }
+  if (g_h0 && at.chunk == 0 && at.group == 0 && at.active) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) g_h0[sc + v] = q.ok ? carry[v] : __builtin_nanf("");
+  }
+}
+
+// How a call is divided.  A workgroup walks a whole sequence at 64 channels a go, unless that leaves the 256 CUs without two workgroups
+// each, or one long sequence would still be walked when the others are done: then sequences are cut into chunks.
+struct Plan {
+  int v, lane_bits, n_chunks, per_row;
+  int64_t chunk;
+};
+
+Plan scan_plan(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max_len, int v) {
+  Plan p;
+  p.v = v;
+  const int lanes_needed = (n_channels + v - 1) / v;
+  p.lane_bits = lanes_needed > 32 ? 6 : lanes_needed > 16 ? 5 : 4;
+  p.per_row = (lanes_needed + (1 << p.lane_bits) - 1) >> p.lane_bits;
+  const int64_t tile = (int64_t)(kThreads >> p.lane_bits) * kSteps, tiles = max_len > 0 ? (max_len + tile - 1) / tile : 1;
+  const int64_t rows = (int64_t)n_seqs * p.per_row;
+  int64_t all = (n_tokens + tile - 1) / tile * p.per_row;  // tiles of the whole call, if its sequences fill them
+  if (all > rows * tiles) all = rows * tiles;
+  // a workgroup's fair share of tiles, over four workgroups a CU, and at least four of them
+  int64_t share = (all + 1023) / 1024;
+  if (share < 4) share = 4;
+  p.n_chunks = 1;
+  if (tiles > 2 * share) {
+    int64_t c = (tiles + share - 1) / share;
+    const int64_t most = rows > 0 ? (1 << 18) / rows : 1;  // short sequences have as many chunks as the longest: mostly empty workgroups
+    if (c > 1024) c = 1024;
+    if (c > most) c = most > 1 ? most : 1;
+    share = (tiles + c - 1) / c;
+    p.n_chunks = (int)((tiles + share - 1) / share);
+  } else {
+    share = tiles;
+  }
+  p.chunk = share * tile;
+  return p;
+}
+
+// V channels per lane: two where 16-bit rows are even and aligned to both
+inline int channels_per_lane(int32_t dtype, int32_t n_channels, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
+  if (dtype == DC_DTYPE_F32 || n_channels % 2) return 1;
+  for (const void* p : ptrs)
+    if (!aligned(p, 4)) return 1;
+  for (int64_t s : strides)
+    if (s % 2) return 1;
+  return 2;
+}
+
+// calls f with the element type and the channels per lane
+template <typename F>
+int with_lanes(int32_t dtype, int v, F&& f) {
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if constexpr (sizeof(T) == 2) {
+      if (v == 2) return f(t, std::integral_constant<int, 2>{});
+    }
+    return f(t, std::integral_constant<int, 1>{});
+  });
+}
+
 int check_scan(int32_t dtype, const void* x, int64_t x_stride, const void* f, int64_t f_stride, int64_t n_tokens, int32_t n_channels,
-               const int64_t* begin, const int64_t* end, int32_t n_seqs, int64_t max_len) {
+               const int64_t* begin, const int64_t* end, int32_t n_seqs, int64_t max_len, const void* workspace, int64_t workspace_bytes) {
   DC_REQUIRE(dtype_ok(dtype), "unknown element type");
   DC_REQUIRE(n_tokens >= 0 && n_channels > 0 && n_seqs >= 0 && max_len >= 0, "negative size");
   DC_REQUIRE((begin == nullptr) == (end == nullptr), "begin and end come together");
   DC_REQUIRE(begin || max_len == 0 || n_seqs <= n_tokens / max_len, "dense sequences exceed the tokens");
   DC_REQUIRE(n_tokens == 0 || (x && f), "null pointer");
   DC_REQUIRE(x_stride >= 0 && f_stride >= 0, "negative stride");
-  DC_REQUIRE((int64_t)n_seqs * ((n_channels + 63) / 64) < ((int64_t)1 << 25), "more than 2^25 blocks of 64 channels");
+  DC_REQUIRE(n_channels <= (1 << 24) && (int64_t)n_seqs * ((n_channels + 63) / 64) < ((int64_t)1 << 20), "more than 2^20 blocks of 64 channels");
   DC_REQUIRE(aligned(x, dtype_size(dtype)) && aligned(f, dtype_size(dtype)), "misaligned pointer");
+  const int64_t need = dc_gated_scan_workspace(n_tokens, n_channels, n_seqs, max_len);
+  DC_REQUIRE(workspace_bytes >= need && (need == 0 || workspace) && aligned(workspace, 16), "workspace too small");
   return DC_OK;
 }
 
@@ -136,24 +593,50 @@ extern "C" int64_t dc_gated_scan_saved(int64_t n_tokens, int32_t n_channels) {
   return n_tokens > 0 && n_channels > 0 ? (n_tokens + dc::kTile - 1) / dc::kTile * n_channels : 0;
 }
 
-extern "C" int64_t dc_gated_scan_workspace(int64_t, int32_t, int32_t, int64_t) { return 0; }
+extern "C" int64_t dc_gated_scan_workspace(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max_len) {
+  if (n_tokens <= 0 || n_channels <= 0 || n_seqs <= 0 || max_len <= dc::kShort) return 0;
+  // maps and starts of whichever division the alignment of the tensors allows
+  int64_t most = 0;
+  for (int v = 1; v <= 2; ++v) {
+    const dc::Plan p = dc::scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
+    if (p.n_chunks > 1 && p.n_chunks > most) most = p.n_chunks;
+  }
+  return most ? (int64_t)n_seqs * (3 * most + 1) * n_channels * 4 : 0;
+}
 
 extern "C" int dc_gated_scan(void* stream, int32_t dtype, const void* d_x, int64_t x_stride, const void* d_f, int64_t f_stride,
                              int64_t n_tokens, int32_t n_channels, const int64_t* d_begin, const int64_t* d_end, int32_t n_seqs,
                              int64_t max_len, int32_t reverse, const float* d_h0, void* d_y, int64_t y_stride, int32_t zero_rest,
                              float* d_h_last, float* d_saved, void* d_workspace, int64_t workspace_bytes) {
   using namespace dc;
-  if (int rc = check_scan(dtype, d_x, x_stride, d_f, f_stride, n_tokens, n_channels, d_begin, d_end, n_seqs, max_len)) return rc;
+  if (int rc = check_scan(dtype, d_x, x_stride, d_f, f_stride, n_tokens, n_channels, d_begin, d_end, n_seqs, max_len, d_workspace, workspace_bytes)) return rc;
   DC_REQUIRE(n_tokens == 0 || d_y, "null pointer");
   DC_REQUIRE(y_stride >= n_channels, "rows of the output overlap");
   DC_REQUIRE(aligned(d_y, dtype_size(dtype)), "misaligned pointer");
-  (void)d_workspace, (void)workspace_bytes;
-  const ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse};
-  return with_dtype(dtype, [&](auto t) {
+  const int v = channels_per_lane(dtype, n_channels, {d_x, d_f, d_y}, {x_stride, f_stride, y_stride});
+  const Plan p = scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
+  ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0};
+  const int zeros = zero_rest && n_tokens > 0 ? kZeroBlocks : 0;
+  return with_lanes(dtype, v, [&](auto t, auto lanes) {
     using T = decltype(t);
-    if (zero_rest && n_tokens > 0) zero_rest_kernel<T><<<dim3(64), dim3(256), 0, as_stream(stream)>>>(a, (T*)d_y, y_stride, nullptr, 0);
-    if (n_seqs > 0) scan_walk_kernel<T><<<dim3(n_seqs * ((n_channels + 63) / 64)), dim3(64), 0, as_stream(stream)>>>(
-        a, (const T*)d_x, x_stride, (const T*)d_f, f_stride, d_h0, (T*)d_y, y_stride, d_h_last, d_saved);
+    constexpr int V = decltype(lanes)::value;
+    const T *x = (const T*)d_x, *f = (const T*)d_f;
+    if (max_len <= kShort) {
+      a.n_blocks = n_seqs * ((n_channels + kWalkThreads * V - 1) / (kWalkThreads * V));
+      if (a.n_blocks + zeros == 0) return DC_OK;
+      scan_walk_kernel<T, V><<<dim3(a.n_blocks + zeros), dim3(kWalkThreads), 0, as_stream(stream)>>>(a, x, x_stride, f, f_stride, d_h0, (T*)d_y, y_stride, d_h_last);
+      DC_LAUNCH_CHECK();
+      return DC_OK;
+    }
+    a.n_blocks = n_seqs * p.per_row * p.n_chunks;
+    if (a.n_blocks + zeros == 0) return DC_OK;
+    float* maps = p.n_chunks > 1 ? (float*)d_workspace : nullptr;
+    if (maps) {
+      scan_map_kernel<T, V, false><<<dim3(a.n_blocks), dim3(kThreads), 0, as_stream(stream)>>>(a, f, f_stride, x, x_stride, d_h0, maps);
+      DC_LAUNCH_CHECK();
+    }
+    scan_tile_kernel<T, V><<<dim3(a.n_blocks + zeros), dim3(kThreads), 0, as_stream(stream)>>>(a, x, x_stride, f, f_stride, d_h0, (T*)d_y, y_stride, d_h_last,
+                                                                                               d_saved, maps);
     DC_LAUNCH_CHECK();
     return DC_OK;
   });
@@ -165,19 +648,37 @@ extern "C" int dc_gated_scan_backward(void* stream, int32_t dtype, const void* d
                                       int64_t grad_y_stride, const float* d_grad_h_last, void* d_grad_x, int64_t grad_x_stride, void* d_grad_f,
                                       int64_t grad_f_stride, int32_t zero_rest, float* d_grad_h0, void* d_workspace, int64_t workspace_bytes) {
   using namespace dc;
-  if (int rc = check_scan(dtype, d_x, x_stride, d_f, f_stride, n_tokens, n_channels, d_begin, d_end, n_seqs, max_len)) return rc;
+  if (int rc = check_scan(dtype, d_x, x_stride, d_f, f_stride, n_tokens, n_channels, d_begin, d_end, n_seqs, max_len, d_workspace, workspace_bytes)) return rc;
   DC_REQUIRE(n_tokens == 0 || (d_saved && d_grad_y && d_grad_x && d_grad_f), "null pointer");
   DC_REQUIRE(grad_y_stride >= 0, "negative stride");
   DC_REQUIRE(grad_x_stride >= n_channels && grad_f_stride >= n_channels, "rows of an output overlap");
   DC_REQUIRE(aligned(d_grad_y, dtype_size(dtype)) && aligned(d_grad_x, dtype_size(dtype)) && aligned(d_grad_f, dtype_size(dtype)), "misaligned pointer");
-  (void)d_workspace, (void)workspace_bytes;
-  const ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse};
-  return with_dtype(dtype, [&](auto t) {
+  const int v = channels_per_lane(dtype, n_channels, {d_x, d_f, d_grad_y, d_grad_x, d_grad_f}, {x_stride, f_stride, grad_y_stride, grad_x_stride, grad_f_stride});
+  const Plan p = scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
+  ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0};
+  const int zeros = zero_rest && n_tokens > 0 ? kZeroBlocks : 0;
+  return with_lanes(dtype, v, [&](auto t, auto lanes) {
     using T = decltype(t);
-    if (zero_rest && n_tokens > 0) zero_rest_kernel<T><<<dim3(64), dim3(256), 0, as_stream(stream)>>>(a, (T*)d_grad_x, grad_x_stride, (T*)d_grad_f, grad_f_stride);
-    if (n_seqs > 0) scan_walk_backward_kernel<T><<<dim3(n_seqs * ((n_channels + 63) / 64)), dim3(64), 0, as_stream(stream)>>>(
-        a, (const T*)d_x, x_stride, (const T*)d_f, f_stride, d_h0, d_saved, (const T*)d_grad_y, grad_y_stride, d_grad_h_last, (T*)d_grad_x,
-        grad_x_stride, (T*)d_grad_f, grad_f_stride, d_grad_h0);
+    constexpr int V = decltype(lanes)::value;
+    const T *x = (const T*)d_x, *f = (const T*)d_f, *gy = (const T*)d_grad_y;
+    T *gx = (T*)d_grad_x, *gf = (T*)d_grad_f;
+    if (max_len <= kShort) {
+      a.n_blocks = n_seqs * ((n_channels + kWalkThreads * V - 1) / (kWalkThreads * V));
+      if (a.n_blocks + zeros == 0) return DC_OK;
+      scan_walk_backward_kernel<T, V><<<dim3(a.n_blocks + zeros), dim3(kWalkThreads), 0, as_stream(stream)>>>(
+          a, x, x_stride, f, f_stride, d_h0, gy, grad_y_stride, d_grad_h_last, gx, grad_x_stride, gf, grad_f_stride, d_grad_h0);
+      DC_LAUNCH_CHECK();
+      return DC_OK;
+    }
+    a.n_blocks = n_seqs * p.per_row * p.n_chunks;
+    if (a.n_blocks + zeros == 0) return DC_OK;
+    float* maps = p.n_chunks > 1 ? (float*)d_workspace : nullptr;
+    if (maps) {
+      scan_map_kernel<T, V, true><<<dim3(a.n_blocks), dim3(kThreads), 0, as_stream(stream)>>>(a, f, f_stride, gy, grad_y_stride, d_grad_h_last, maps);
+      DC_LAUNCH_CHECK();
+    }
+    scan_tile_backward_kernel<T, V><<<dim3(a.n_blocks + zeros), dim3(kThreads), 0, as_stream(stream)>>>(
+        a, x, x_stride, f, f_stride, d_h0, d_saved, gy, grad_y_stride, d_grad_h_last, gx, grad_x_stride, gf, grad_f_stride, d_grad_h0, maps);
     DC_LAUNCH_CHECK();
     return DC_OK;
   });

@@ -466,7 +466,7 @@ int dc_gated_scan(void* stream, int32_t dtype, const void* d_x, int64_t x_stride
                   int64_t max_len, int32_t reverse, const float* d_h0, void* d_y, int64_t y_stride, int32_t zero_rest,
                   float* d_h_last, float* d_saved, void* d_workspace, int64_t workspace_bytes);
 int64_t dc_gated_scan_workspace(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max_len);
-/* floats of d_saved: the state on entering every 128-token tile of [0, n_tokens) */
+/* floats of d_saved: the states between the 64-token tiles of the sequences */
 int64_t dc_gated_scan_saved(int64_t n_tokens, int32_t n_channels);
 
 /* Its backward pass.  With g_t = dy_t + a_(t+1) g_(t+1), plus d_grad_h_last at the last token:

@@ -62,7 +62,7 @@ def test_gated_scan_refusals(L):
     refused(L, scan(L, xs=-1), "negative stride")
     refused(L, scan(L, ys=7), "overlap")
     refused(L, scan(L, x=ODD), "misaligned")
-    refused(L, scan(L, seqs=1 << 30, c=256), "2^25")
+    refused(L, scan(L, seqs=1 << 30, c=256), "2^20")
     back = lambda saved=P, gy=P, gx=P, gxs=8, gf=P: L.dc_gated_scan_backward(  # noqa: E731
         None, 0, P, 8, P, 8, 100, 8, P, P, 2, 50, 0, None, saved, gy, 8, None, gx, gxs, gf, 8, 0, None, P, 1 << 30)
     refused(L, back(saved=None), "null pointer")
@@ -70,8 +70,8 @@ def test_gated_scan_refusals(L):
     refused(L, back(gf=None), "null pointer")
     refused(L, back(gxs=5), "overlap")
     refused(L, back(gx=ODD), "misaligned")
-    assert L.dc_gated_scan_saved(0, 8) == 0 and L.dc_gated_scan_saved(1, 8) == 8 and L.dc_gated_scan_saved(129, 8) == 16
-    assert L.dc_gated_scan_saved(1 << 33, 256) == 1 << 34
+    assert L.dc_gated_scan_saved(0, 8) == 0 and L.dc_gated_scan_saved(1, 8) == 8 and L.dc_gated_scan_saved(65, 8) == 16
+    assert L.dc_gated_scan_saved(1 << 33, 256) == 1 << 35
 
 
 def norm(L, dtype=0, rdtype=0, n=4, w=8, kind=0, eps=1e-5, y=P, g=P, act=1, r=P, out=P, outs=8, normed=P):
