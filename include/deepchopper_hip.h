@@ -417,7 +417,7 @@ int dc_model_profile_stages(dc_model* m, char* buf, int32_t buf_len);
 #define DC_ACT_SIGMOID 1
 #define DC_ACT_SILU 2
 #define DC_MAX_TOP 32            /* most alternatives dc_token_logprobs reports                              */
-#define DC_MAX_NORM_WIDTH 16384  /* widest row of dc_block_norm                                              */
+#define DC_MAX_NORM_WIDTH 8192   /* widest row of dc_block_norm                                              */
 #define DC_STATS_FROM 513        /* classes from which dc_token_logprobs_backward takes the forward's d_stats */
 
 /* Log probabilities of given tokens, entropy and top alternatives.  Row i, with m = max_j z_ij and S = sum_j exp(z_ij - m):

@@ -84,7 +84,7 @@ def test_block_norm_refusals(L):
     refused(L, norm(L, rdtype=1), "residual stream")
     refused(L, norm(L, n=-1), "negative size")
     refused(L, norm(L, w=0), "width")
-    refused(L, norm(L, w=16385), "width")
+    refused(L, norm(L, w=8193), "width")
     refused(L, norm(L, kind=2), "unknown norm")
     refused(L, norm(L, act=3), "activation")
     refused(L, norm(L, eps=-1.0), "eps")
@@ -99,7 +99,7 @@ def test_block_norm_refusals(L):
     refused(L, back(ws=None), "workspace")
     refused(L, back(nb=L.dc_block_norm_workspace(4, 8) - 1), "workspace")
     refused(L, back(ws=C.c_void_p(4100)), "workspace")
-    assert L.dc_block_norm_workspace(0, 8) == 0 and L.dc_block_norm_workspace(1 << 40, 16384) < 1 << 31
+    assert L.dc_block_norm_workspace(0, 8) == 0 and L.dc_block_norm_workspace(1 << 40, 8192) < 1 << 31
     assert norm(L, n=0) == 0 and norm(L, out=None, normed=None) == 0
 
 
