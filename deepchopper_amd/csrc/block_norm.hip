@@ -28,104 +28,177 @@ struct NormArgs {
 };
 
 __device__ __forceinline__ float sigmoid(float x) { return fast_rcp(1.0f + fast_exp2(-x * kLog2e)); }
-__device__ __forceinline__ float act_of(int act, float x) {
-  return act == DC_ACT_IDENTITY ? x : act == DC_ACT_SIGMOID ? sigmoid(x) : x * sigmoid(x);
-}
 
 // One row's columns of this thread: K vectors of V, 256 * n_waves apart.  Elements beyond the width are 0 and not stored.
 template <int K>
 struct Part {
   float v[K][V];
 };
+// ... as they lie in memory: the next row is on its way while one is worked on
+template <typename T, int K>
+struct RawPart {
+  typename loose_vec<T, V>::type r[K];
+};
 
-// Where a thread's columns and rows lie.
+// How a row lies in a workgroup: several rows in a wavefront (at most 128 columns), a row in one, a row in several.
+enum Form { kSub, kWave, kTeam };
+
+// Where a thread's columns and rows lie.  Outside kSub the row is the wavefront's, kept in scalar registers.
+template <Form F>
 struct Spot {
-  int lane, column, step, group, n_groups;  // first column, columns between vectors, row group of the workgroup
+  int column, step, wave, group, n_groups;  // first column, columns between vectors, row group of the workgroup
   __device__ __forceinline__ Spot(const NormArgs& a) {
-    const int wave = threadIdx.x >> 6, per_row = a.n_waves;
-    if (per_row == 1) {
-      lane = threadIdx.x & ((1 << a.lane_bits) - 1);
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if constexpr (F == kSub) {
+      column = (threadIdx.x & ((1 << a.lane_bits) - 1)) * V;
       group = threadIdx.x >> a.lane_bits;
       n_groups = blockDim.x >> a.lane_bits;
-      column = lane * V;
     } else {
-      lane = threadIdx.x & 63;
+      const int per_row = F == kTeam ? a.n_waves : 1;
+      column = (wave % per_row * 64 + (threadIdx.x & 63)) * V;
       group = wave / per_row;
       n_groups = (int)(blockDim.x >> 6) / per_row;
-      column = (wave % per_row * 64 + lane) * V;
     }
-    step = per_row * 64 * V;
+    step = a.n_waves * 64 * V;
   }
 };
 
-template <int K, typename T>
-__device__ __forceinline__ void load_part(const T* row, const NormArgs& a, const Spot& at, Part<K>& p) {
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = at.column + k * at.step;
-    if (c + V <= a.width) {
-      load_vec<V>(row + c, p.v[k]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) p.v[k][i] = c + i < a.width ? (float)row[c + i] : 0.0f;
-    }
-  }
-}
-template <int K, typename T>
-__device__ __forceinline__ void store_part(T* row, const NormArgs& a, const Spot& at, const Part<K>& p) {
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = at.column + k * at.step;
-    if (c + V <= a.width) {
-      store_vec<V>(row + c, p.v[k]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (c + i < a.width) row[c + i] = (T)p.v[k][i];
-    }
-  }
-}
-// a vector of the width, or a constant
+// columns that wavefront w of a row has
 template <int K>
-__device__ __forceinline__ void load_weights(const float* w, float other, const NormArgs& a, const Spot& at, Part<K>& p) {
-  if (w) {
-    load_part<K>(w, a, at, p);
-  } else {
+__device__ __forceinline__ float columns_of(const NormArgs& a, int w) {
+  int n = 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+  for (int k = 0; k < K; ++k) {
+    const int left = a.width - (w + k * a.n_waves) * 64 * V;
+    n += left < 0 ? 0 : left < 64 * V ? left : 64 * V;
+  }
+  return (float)n;
+}
+
+// the thread's whole vectors of a row, or the single elements of the one that the width cuts
+template <typename T, int K>
+__device__ __forceinline__ void load_whole(const T* row, int c, int k, RawPart<T, K>& p) {
+  p.r[k] = *reinterpret_cast<const typename loose_vec<T, V>::type*>(row + c);
+}
+template <typename T, int K>
+__device__ __forceinline__ void load_cut(const T* row, int c, int k, int width, RawPart<T, K>& p) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) p.v[k][i] = other;
+  for (int i = 0; i < V - 1; ++i)
+    if (c + i < width) p.r[k][i] = row[c + i];
+}
+template <typename T, int K>
+__device__ __forceinline__ void clear(RawPart<T, K>& p) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) p.r[k][i] = (T)0.0f;
+}
+template <typename T, int K>
+__device__ __forceinline__ void store_whole(T* row, int c, int k, const Part<K>& p) {
+  store_vec<V>(row + c, p.v[k]);
+}
+template <typename T, int K>
+__device__ __forceinline__ void store_cut(T* row, int c, int k, int width, const Part<K>& p) {
+#pragma unroll
+  for (int i = 0; i < V - 1; ++i)
+    if (c + i < width) row[c + i] = (T)p.v[k][i];
+}
+// f(whole, c, k) for every vector of the thread that has elements of the row
+template <int K, typename At, typename Fn>
+__device__ __forceinline__ void for_vectors(const NormArgs& a, const At& at, Fn&& f) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = at.column + k * at.step;
+    if (c + V <= a.width) f(std::true_type{}, c, k);
+    else if (c < a.width) f(std::false_type{}, c, k);
+  }
+}
+template <typename T, int K>
+__device__ __forceinline__ void widen(const RawPart<T, K>& p, Part<K>& out) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) out.v[k][i] = (float)p.r[k][i];
+}
+// The gate's activation, in place; with `slope`, its derivative.
+template <int K>
+__device__ __forceinline__ void activate(const NormArgs& a, Part<K>& g, Part<K>* slope) {
+  if (a.act == DC_ACT_IDENTITY) {
+    if (slope) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) slope->v[k][i] = 1.0f;
+    }
+    return;
+  }
+  const bool silu = a.act == DC_ACT_SILU;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float x = g.v[k][i], s = sigmoid(x);
+      if (slope) slope->v[k][i] = s * (silu ? __builtin_fmaf(x, 1.0f - s, 1.0f) : 1.0f - s);
+      g.v[k][i] = silu ? x * s : s;
+    }
+  }
+}
+template <int K>
+__device__ __forceinline__ void fill(Part<K>& p, float x) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i) p.v[k][i] = x;
+}
+// a vector of the width, or a constant; 0 beyond the width, which keeps what stands there out of every sum
+template <int K, typename At>
+__device__ __forceinline__ void load_weights(const float* w, float other, const NormArgs& a, const At& at, Part<K>& p) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = at.column + k * at.step + i;
+      p.v[k][i] = c >= a.width ? 0.0f : w ? w[c] : other;
+    }
   }
 }
 
-// Sum over the row.  MULTI: its wavefronts meet in `scratch` (one slot a wavefront, two halves used in turn: one barrier a sum).
-template <bool MULTI>
-__device__ __forceinline__ float row_sum(float v, const NormArgs& a, float (*scratch)[16], int& turn) {
-  v = lanes_sum(v, MULTI ? 6 : a.lane_bits);
-  if constexpr (MULTI) {
-    const int wave = threadIdx.x >> 6, first = wave / a.n_waves * a.n_waves;
-    if ((threadIdx.x & 63) == 0) scratch[turn][wave] = v;
+// What the wavefronts of a row tell each other, one slot a wavefront, two halves used in turn: one barrier an exchange.
+struct Meeting {
+  float2 slot[2][16];
+};
+
+// Sums over the row of one or two values.
+template <Form F>
+__device__ __forceinline__ float2 row_sums(float x, float y, bool two, const NormArgs& a, const Spot<F>& at, Meeting& m, int& turn) {
+  const int bits = F == kSub ? a.lane_bits : 6;
+  float2 s{lanes_sum(x, bits), two ? lanes_sum(y, bits) : 0.0f};
+  if constexpr (F == kTeam) {
+    const int first = at.group * a.n_waves;
+    if ((threadIdx.x & 63) == 0) m.slot[turn][at.wave] = s;
     __syncthreads();
-    v = scratch[turn][first];
-    for (int w = 1; w < a.n_waves; ++w) v += scratch[turn][first + w];
+    s = m.slot[turn][first];
+    for (int w = 1; w < a.n_waves; ++w) s.x += m.slot[turn][first + w].x, s.y += m.slot[turn][first + w].y;
     turn ^= 1;
   }
-  return v;
+  return s;
 }
 
-// mean (RMS: 0) and 1 / deviation of a row; elements beyond the width are 0
-template <int K, bool MULTI>
-__device__ __forceinline__ float2 row_stats(const Part<K>& p, const NormArgs& a, const Spot& at, float (*scratch)[16], int& turn) {
-  float mean = 0.0f;
+// mean (RMS: 0) and 1 / deviation of a row; elements beyond the width are 0.  The squares are taken about the mean: of the wavefront's own
+// columns first, moved to the row's mean when the wavefronts meet (sum (x - m)^2 = sum (x - m_w)^2 + n_w (m_w - m)^2).
+template <int K, Form F>
+__device__ __forceinline__ float2 row_stats(const Part<K>& p, const NormArgs& a, const Spot<F>& at, Meeting& m, int& turn) {
+  const int bits = F == kSub ? a.lane_bits : 6;
+  float mean = 0.0f, q = 0.0f;
   if (a.kind == DC_NORM_LAYER) {
     float s = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int i = 0; i < V; ++i) s += p.v[k][i];
-    mean = row_sum<MULTI>(s, a, scratch, turn) * a.inv_width;
+    s = lanes_sum(s, bits);
+    mean = F == kTeam ? s * fast_rcp(__builtin_fmaxf(columns_of<K>(a, at.wave - at.group * a.n_waves), 1.0f)) : s * a.inv_width;
   }
-  float q = 0.0f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = at.column + k * at.step;
@@ -135,198 +208,276 @@ __device__ __forceinline__ float2 row_stats(const Part<K>& p, const NormArgs& a,
       q = __builtin_fmaf(d, d, q);
     }
   }
-  return {mean, 1.0f / sqrtf(row_sum<MULTI>(q, a, scratch, turn) * a.inv_width + a.eps)};
+  q = lanes_sum(q, bits);
+  if constexpr (F == kTeam) {
+    const int first = at.group * a.n_waves;
+    if ((threadIdx.x & 63) == 0) m.slot[turn][at.wave] = {mean, q};
+    __syncthreads();
+    q = 0.0f;
+    if (a.kind == DC_NORM_LAYER) {
+      float all = 0.0f;
+      for (int w = 0; w < a.n_waves; ++w) all = __builtin_fmaf(m.slot[turn][first + w].x, columns_of<K>(a, w), all);
+      all *= a.inv_width;
+      for (int w = 0; w < a.n_waves; ++w) {
+        const float2 o = m.slot[turn][first + w];
+        q += __builtin_fmaf((o.x - all) * (o.x - all), columns_of<K>(a, w), o.y);
+      }
+      mean = all;
+    } else {
+      for (int w = 0; w < a.n_waves; ++w) q += m.slot[turn][first + w].y;
+    }
+    turn ^= 1;
+  }
+  return {mean, __builtin_amdgcn_rsqf(__builtin_fmaf(q, a.inv_width, a.eps))};  // (v_rsq_f32: 1 ulp)
 }
 
-constexpr int kMaxThreads = 1024;
+// The rows of a workgroup's group: blockIdx.x * n_groups + group, ...; all groups take the same number of turns (a team's sums have
+// barriers), one without a row in the last turn works on the last row again and stores nothing.
+struct Rows {
+  int64_t first, step, n;
+  int group;
+  template <Form F>
+  __device__ __forceinline__ Rows(const NormArgs& a, const Spot<F>& at)
+      : first((int64_t)blockIdx.x * at.n_groups), step((int64_t)gridDim.x * at.n_groups), n(a.n_rows), group(at.group) {}
+  __device__ __forceinline__ int64_t clamped(int64_t f) const { return f + group < n ? f + group : n - 1; }
+};
 
-template <typename T, typename R, int K, bool MULTI>
-__global__ __launch_bounds__(MULTI ? kMaxThreads : 256) void block_norm_kernel(NormArgs a, const T* y, const T* gate, const R* residual, R* residual_out,
+template <typename T, typename R, int K, Form F, int THREADS>
+__global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a, const T* y, const T* gate, const R* residual, R* residual_out,
                                                                               int64_t residual_out_stride, T* normed, int64_t normed_stride) {
-  __shared__ float scratch[2][16];
+  __shared__ Meeting meeting;
   int turn = 0;
-  const Spot at(a);
+  const Spot<F> at(a);
+  const Rows rows(a, at);
+  RawPart<T, K> raw_y, raw_g;
+  RawPart<R, K> raw_r;
+  clear(raw_y), clear(raw_g), clear(raw_r);
+  auto fetch = [&](int64_t row) {
+    const T *py = y + row * a.y_stride, *pg = gate + row * a.gate_stride;
+    const R* pr = residual + row * a.residual_stride;
+    for_vectors<K>(a, at, [&](auto whole, int c, int k) {
+      if constexpr (decltype(whole)::value) {
+        if (y) load_whole(py, c, k, raw_y);
+        if (gate) load_whole(pg, c, k, raw_g);
+        if (residual) load_whole(pr, c, k, raw_r);
+      } else {
+        if (y) load_cut(py, c, k, a.width, raw_y);
+        if (gate) load_cut(pg, c, k, a.width, raw_g);
+        if (residual) load_cut(pr, c, k, a.width, raw_r);
+      }
+    });
+  };
+  if (rows.first < rows.n) fetch(rows.clamped(rows.first));
   Part<K> sc, w1, b1, w2, b2;
   load_weights(a.scale, 1.0f, a, at, sc);
   load_weights(a.post_w, 1.0f, a, at, w1);
   load_weights(a.post_b, 0.0f, a, at, b1);
   load_weights(a.pre_w, 1.0f, a, at, w2);
   load_weights(a.pre_b, 0.0f, a, at, b2);
-  // (all row groups of a workgroup take the same number of turns: a MULTI row sum has barriers)
-  for (int64_t first = (int64_t)blockIdx.x * at.n_groups; first < a.n_rows; first += (int64_t)gridDim.x * at.n_groups) {
-    const int64_t row = first + at.group;
-    const bool live = row < a.n_rows;
-    const int64_t r0 = live ? row : a.n_rows - 1;  // a group without a row reads the last one
+  for (int64_t f = rows.first; f < rows.n; f += rows.step) {
+    const int64_t row = f + at.group;
+    const bool live = row < rows.n;
     Part<K> v, g, r;
-    if (y) load_part<K>(y + r0 * a.y_stride, a, at, v);
-    if (gate) load_part<K>(gate + r0 * a.gate_stride, a, at, g);
-    if (residual) load_part<K>(residual + r0 * a.residual_stride, a, at, r);
-    else load_weights<K>(nullptr, 0.0f, a, at, r);
+    fill(r, 0.0f);
+    if (y) widen(raw_y, v);
+    if (gate) widen(raw_g, g);
+    if (residual) widen(raw_r, r);
+    if (f + rows.step < rows.n) fetch(rows.clamped(f + rows.step));
     if (y) {
+      if (gate) activate<K>(a, g, nullptr);
+      else fill(g, 1.0f);
       float2 st{0.0f, 1.0f};
-      if (a.post_norm) st = row_stats<K, MULTI>(v, a, at, scratch, turn);
+      if (a.post_norm) st = row_stats<K, F>(v, a, at, meeting, turn);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = at.column + k * at.step;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           float u = v.v[k][i];
           if (a.post_norm) u = __builtin_fmaf((u - st.x) * st.y, w1.v[k][i], b1.v[k][i]);
-          if (gate) u *= act_of(a.act, g.v[k][i]);
-          r.v[k][i] = c + i < a.width ? __builtin_fmaf(sc.v[k][i], u, r.v[k][i]) : 0.0f;
+          r.v[k][i] = __builtin_fmaf(sc.v[k][i], g.v[k][i] * u, r.v[k][i]);
         }
       }
     }
-    if (residual_out && live) store_part<K>(residual_out + row * residual_out_stride, a, at, r);
     if (normed) {
-      const float2 st = row_stats<K, MULTI>(r, a, at, scratch, turn);
+      const float2 st = row_stats<K, F>(r, a, at, meeting, turn);
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) r.v[k][i] = __builtin_fmaf((r.v[k][i] - st.x) * st.y, w2.v[k][i], b2.v[k][i]);
-      if (live) store_part<K>(normed + row * normed_stride, a, at, r);
+        for (int i = 0; i < V; ++i) v.v[k][i] = __builtin_fmaf((r.v[k][i] - st.x) * st.y, w2.v[k][i], b2.v[k][i]);
     }
+    if (!live) continue;
+    R* po = residual_out + row * residual_out_stride;
+    T* pn = normed + row * normed_stride;
+    for_vectors<K>(a, at, [&](auto whole, int c, int k) {
+      if constexpr (decltype(whole)::value) {
+        if (residual_out) store_whole(po, c, k, r);
+        if (normed) store_whole(pn, c, k, v);
+      } else {
+        if (residual_out) store_cut(po, c, k, a.width, r);
+        if (normed) store_cut(pn, c, k, a.width, v);
+      }
+    });
   }
 }
 
 // The gradient g of a normalised row, in place, to that of the row: factor (g - mean(g) - hat mean(g hat)).
-template <int K, bool MULTI>
-__device__ __forceinline__ void norm_back(Part<K>& g, const Part<K>& hat, const NormArgs& a, float factor, float (*scratch)[16], int& turn) {
+template <int K, Form F>
+__device__ __forceinline__ void norm_back(Part<K>& g, const Part<K>& hat, const NormArgs& a, const Spot<F>& at, float factor, Meeting& m, int& turn) {
   float s = 0.0f, q = 0.0f;
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int i = 0; i < V; ++i) s += g.v[k][i], q = __builtin_fmaf(g.v[k][i], hat.v[k][i], q);
-  s = a.kind == DC_NORM_LAYER ? row_sum<MULTI>(s, a, scratch, turn) * a.inv_width : 0.0f;
-  q = row_sum<MULTI>(q, a, scratch, turn) * a.inv_width;
+  const bool layer = a.kind == DC_NORM_LAYER;
+  const float2 t = row_sums<F>(q, s, layer, a, at, m, turn);
+  q = t.x * a.inv_width;
+  s = layer ? t.y * a.inv_width : 0.0f;
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int i = 0; i < V; ++i) g.v[k][i] = factor * (g.v[k][i] - s - hat.v[k][i] * q);
 }
 
-// Rows blockIdx.x * groups + group, ... ; the workgroup's sums over them, [5][width] in the order scale, post_w, post_b, pre_w, pre_b,
-// go to sums[blockIdx.x].
-template <typename T, typename R, int K, bool MULTI>
-__global__ __launch_bounds__(MULTI ? kMaxThreads : 256) void block_norm_backward_kernel(NormArgs a, const T* y, const T* gate, const R* residual,
+// Rows as in the forward pass; the workgroup's sums over them, [5][width] in the order scale, post_w, post_b, pre_w, pre_b, go to
+// sums[blockIdx.x].
+template <typename T, typename R, int K, Form F, int THREADS>
+__global__ __launch_bounds__(THREADS) void block_norm_backward_kernel(NormArgs a, const T* y, const T* gate, const R* residual,
                                                                                        const R* g_out, int64_t g_out_stride, const T* g_normed,
                                                                                        int64_t g_normed_stride, T* g_y, T* g_gate, R* g_residual,
                                                                                        float* __restrict__ sums) {
   extern __shared__ float lds[];  // one vector per row group
-  __shared__ float scratch[2][16];
+  __shared__ Meeting meeting;
   int turn = 0;
-  const Spot at(a);
-  Part<K> acc[5];
+  const Spot<F> at(a);
+  const Rows rows(a, at);
+  RawPart<T, K> raw_y, raw_g, raw_n;
+  RawPart<R, K> raw_r, raw_o;
+  clear(raw_y), clear(raw_g), clear(raw_n), clear(raw_r), clear(raw_o);
+  auto fetch = [&](int64_t row) {
+    const T *py = y + row * a.y_stride, *pg = gate + row * a.gate_stride, *pn = g_normed + row * g_normed_stride;
+    const R *pr = residual + row * a.residual_stride, *po = g_out + row * g_out_stride;
+    for_vectors<K>(a, at, [&](auto whole, int c, int k) {
+      if constexpr (decltype(whole)::value) {
+        if (y) load_whole(py, c, k, raw_y);
+        if (residual) load_whole(pr, c, k, raw_r);
+        if (gate) load_whole(pg, c, k, raw_g);
+        if (g_normed) load_whole(pn, c, k, raw_n);
+        if (g_out) load_whole(po, c, k, raw_o);
+      } else {
+        if (y) load_cut(py, c, k, a.width, raw_y);
+        if (residual) load_cut(pr, c, k, a.width, raw_r);
+        if (gate) load_cut(pg, c, k, a.width, raw_g);
+        if (g_normed) load_cut(pn, c, k, a.width, raw_n);
+        if (g_out) load_cut(po, c, k, a.width, raw_o);
+      }
+    });
+  };
+  if (rows.first < rows.n) fetch(rows.clamped(rows.first));
+  Part<K> acc[5], sc, w1, b1, w2;
 #pragma unroll
-  for (int n = 0; n < 5; ++n) load_weights<K>(nullptr, 0.0f, a, at, acc[n]);
-  for (int64_t first = (int64_t)blockIdx.x * at.n_groups; first < a.n_rows; first += (int64_t)gridDim.x * at.n_groups) {
-    const int64_t row = first + at.group;
-    const bool live = row < a.n_rows;
-    const int64_t r0 = live ? row : a.n_rows - 1;
-    const float on = live ? 1.0f : 0.0f;  // (a group without a row adds nothing)
-    Part<K> hat, g, t, r, w;
+  for (int n = 0; n < 5; ++n) fill(acc[n], 0.0f);
+  load_weights(a.scale, 1.0f, a, at, sc);
+  load_weights(a.post_w, 1.0f, a, at, w1);
+  load_weights(a.post_b, 0.0f, a, at, b1);
+  load_weights(a.pre_w, 1.0f, a, at, w2);
+  for (int64_t f = rows.first; f < rows.n; f += rows.step) {
+    const int64_t row = f + at.group;
+    const bool live = row < rows.n;
+    Part<K> hat, g, slope, t, r, o;  // g: act(gate)
+    fill(r, 0.0f);
+    fill(o, 0.0f);
+    if (y) widen(raw_y, hat);
+    if (residual) widen(raw_r, r);
+    if (gate) widen(raw_g, g);
+    if (g_normed) widen(raw_n, t);
+    if (g_out) widen(raw_o, o);
+    if (f + rows.step < rows.n) fetch(rows.clamped(f + rows.step));
     float2 st{0.0f, 1.0f};
-    if (residual) load_part<K>(residual + r0 * a.residual_stride, a, at, r);
-    else load_weights<K>(nullptr, 0.0f, a, at, r);
-    if (g_normed) load_part<K>(g_normed + r0 * g_normed_stride, a, at, t);
-    if (y) {  // hat: the normalised block output (or the output itself)
-      load_part<K>(y + r0 * a.y_stride, a, at, hat);
-      if (gate) load_part<K>(gate + r0 * a.gate_stride, a, at, g);
+    if (y) {  // hat: the normalised block output (or the output itself); r: r'
+      if (gate) activate<K>(a, g, &slope);
+      else fill(g, 1.0f);
       if (a.post_norm) {
-        st = row_stats<K, MULTI>(hat, a, at, scratch, turn);
+        st = row_stats<K, F>(hat, a, at, meeting, turn);
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int i = 0; i < V; ++i) hat.v[k][i] = (hat.v[k][i] - st.x) * st.y;
       }
-      Part<K> sc, b;
-      load_weights(a.scale, 1.0f, a, at, sc);
-      load_weights(a.post_w, 1.0f, a, at, w);
-      load_weights(a.post_b, 0.0f, a, at, b);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = at.column + k * at.step;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          float u = a.post_norm ? __builtin_fmaf(hat.v[k][i], w.v[k][i], b.v[k][i]) : hat.v[k][i];
-          if (gate) u *= act_of(a.act, g.v[k][i]);
-          r.v[k][i] = c + i < a.width ? __builtin_fmaf(sc.v[k][i], u, r.v[k][i]) : 0.0f;
+          const float u = a.post_norm ? __builtin_fmaf(hat.v[k][i], w1.v[k][i], b1.v[k][i]) : hat.v[k][i];
+          r.v[k][i] = __builtin_fmaf(sc.v[k][i], g.v[k][i] * u, r.v[k][i]);
         }
       }
     }
     if (g_normed) {  // r becomes the normalised r', t the gradient of r' through the norm
-      const float2 st2 = row_stats<K, MULTI>(r, a, at, scratch, turn);
-      load_weights(a.pre_w, 1.0f, a, at, w);
+      const float2 st2 = row_stats<K, F>(r, a, at, meeting, turn);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = at.column + k * at.step;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          r.v[k][i] = c + i < a.width ? (r.v[k][i] - st2.x) * st2.y : 0.0f;
-          acc[3].v[k][i] = __builtin_fmaf(on * t.v[k][i], r.v[k][i], acc[3].v[k][i]);
-          acc[4].v[k][i] = __builtin_fmaf(on, t.v[k][i], acc[4].v[k][i]);
-          t.v[k][i] *= w.v[k][i];
+          r.v[k][i] = (r.v[k][i] - st2.x) * st2.y;
+          if (live) {
+            acc[3].v[k][i] = __builtin_fmaf(t.v[k][i], r.v[k][i], acc[3].v[k][i]);
+            acc[4].v[k][i] += t.v[k][i];
+          }
+          t.v[k][i] *= w2.v[k][i];
         }
       }
-      norm_back<K, MULTI>(t, r, a, st2.y, scratch, turn);
-    } else {
-      load_weights<K>(nullptr, 0.0f, a, at, t);
-    }
-    if (g_out) {
-      load_part<K>(g_out + r0 * g_out_stride, a, at, r);
+      norm_back<K, F>(t, r, a, at, st2.y, meeting, turn);
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) t.v[k][i] += r.v[k][i];
+        for (int i = 0; i < V; ++i) t.v[k][i] += o.v[k][i];
+    } else {
+      t = o;
     }
-    if (g_residual && live) store_part<K>(g_residual + row * a.width, a, at, t);
-    if (!y) continue;
-    Part<K> sc, b;
-    load_weights(a.scale, 1.0f, a, at, sc);
-    load_weights(a.post_w, 1.0f, a, at, w);
-    load_weights(a.post_b, 0.0f, a, at, b);
+    r = t;  // the gradient of the residual
+    if (y) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = at.column + k * at.step;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float u = a.post_norm ? __builtin_fmaf(hat.v[k][i], w.v[k][i], b.v[k][i]) : hat.v[k][i];
+        const float u = a.post_norm ? __builtin_fmaf(hat.v[k][i], w1.v[k][i], b1.v[k][i]) : hat.v[k][i];
         const float gv = t.v[k][i] * sc.v[k][i];
-        float av = 1.0f;
-        if (gate) {
-          const float x = g.v[k][i], s = sigmoid(x);
-          av = a.act == DC_ACT_IDENTITY ? x : a.act == DC_ACT_SIGMOID ? s : x * s;
-          const float slope = a.act == DC_ACT_IDENTITY ? 1.0f : a.act == DC_ACT_SIGMOID ? s * (1.0f - s) : s * (1.0f + x * (1.0f - s));
-          g.v[k][i] = gv * u * slope;
+        const float gu = gv * g.v[k][i];
+        if (live) {
+          acc[0].v[k][i] = __builtin_fmaf(t.v[k][i], g.v[k][i] * u, acc[0].v[k][i]);
+          acc[1].v[k][i] = __builtin_fmaf(gu, hat.v[k][i], acc[1].v[k][i]);
+          acc[2].v[k][i] += gu;
         }
-        const float gu = c + i < a.width ? gv * av : 0.0f;
-        acc[0].v[k][i] = __builtin_fmaf(on * t.v[k][i], av * u, acc[0].v[k][i]);
-        acc[1].v[k][i] = __builtin_fmaf(on * gu, hat.v[k][i], acc[1].v[k][i]);
-        acc[2].v[k][i] = __builtin_fmaf(on, gu, acc[2].v[k][i]);
-        t.v[k][i] = a.post_norm ? gu * w.v[k][i] : gu;
+        slope.v[k][i] *= gv * u;
+        t.v[k][i] = a.post_norm ? gu * w1.v[k][i] : gu;
       }
     }
-    if (gate && g_gate && live) store_part<K>(g_gate + row * a.width, a, at, g);
-    if (g_y) {
-      if (a.post_norm) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const int c = at.column + k * at.step;
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (c + i >= a.width) hat.v[k][i] = 0.0f;
-        }
-        norm_back<K, MULTI>(t, hat, a, st.y, scratch, turn);
-      }
-      if (live) store_part<K>(g_y + row * a.width, a, at, t);
+    if (g_y && a.post_norm) norm_back<K, F>(t, hat, a, at, st.y, meeting, turn);
     }
+    if (!live) continue;
+    R* pr = g_residual + row * a.width;
+    T *pg = g_gate + row * a.width, *py = g_y + row * a.width;
+    for_vectors<K>(a, at, [&](auto whole, int c, int k) {
+      if constexpr (decltype(whole)::value) {
+        if (g_residual) store_whole(pr, c, k, r);
+        if (gate && g_gate) store_whole(pg, c, k, slope);
+        if (y && g_y) store_whole(py, c, k, t);
+      } else {
+        if (g_residual) store_cut(pr, c, k, a.width, r);
+        if (gate && g_gate) store_cut(pg, c, k, a.width, slope);
+        if (y && g_y) store_cut(py, c, k, a.width, t);
+      }
+    });
   }
   if (!sums) return;
   float* own = sums + (int64_t)blockIdx.x * 5 * a.width;
 #pragma unroll
   for (int n = 0; n < 5; ++n) {
     __syncthreads();
-    store_part<K>(lds + at.group * a.width, a, at, acc[n]);
+    for_vectors<K>(a, at, [&](auto whole, int c, int k) {
+      if constexpr (decltype(whole)::value) store_whole(lds + at.group * a.width, c, k, acc[n]);
+      else store_cut(lds + at.group * a.width, c, k, a.width, acc[n]);
+    });
     __syncthreads();
     for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
       float s = lds[c];
@@ -415,8 +566,16 @@ template <typename F>
 int with_row(int32_t dtype, int32_t residual_dtype, const RowPlan& p, F&& f) {
   return with_dtype(dtype, [&](auto t) {
     auto g = [&](auto r) {
-      if (p.k == 1) return p.n_waves > 1 ? f(t, r, std::integral_constant<int, 1>{}, std::true_type{}) : f(t, r, std::integral_constant<int, 1>{}, std::false_type{});
-      return p.n_waves > 1 ? f(t, r, std::integral_constant<int, 2>{}, std::true_type{}) : f(t, r, std::integral_constant<int, 2>{}, std::false_type{});
+      using One = std::integral_constant<int, 1>;
+      using Two = std::integral_constant<int, 2>;
+      using Wave = std::integral_constant<Form, kWave>;
+      using Team = std::integral_constant<Form, kTeam>;
+      using Small = std::integral_constant<int, 256>;
+      using Large = std::integral_constant<int, 1024>;
+      if (p.n_waves == 1 && p.lane_bits < 6) return f(t, r, One{}, std::integral_constant<Form, kSub>{}, Small{});
+      if (p.n_waves == 1) return p.k == 1 ? f(t, r, One{}, Wave{}, Small{}) : f(t, r, Two{}, Wave{}, Small{});
+      if (p.n_waves <= 4) return p.k == 1 ? f(t, r, One{}, Team{}, Small{}) : f(t, r, Two{}, Team{}, Small{});
+      return p.k == 1 ? f(t, r, One{}, Team{}, Large{}) : f(t, r, Two{}, Team{}, Large{});
     };
     return residual_dtype == dtype ? g(t) : g(f32{});
   });
@@ -446,10 +605,10 @@ extern "C" int dc_block_norm(void* stream, int32_t dtype, int32_t residual_dtype
   const int groups = p.n_waves > 1 ? p.threads / 64 / p.n_waves : p.threads >> p.lane_bits;
   const int64_t need = (n_rows + groups - 1) / groups;
   const int grid = (int)(need < 4096 ? need : 4096);
-  return with_row(dtype, residual_dtype, p, [&](auto t, auto r, auto k, auto multi) {
+  return with_row(dtype, residual_dtype, p, [&](auto t, auto r, auto k, auto form, auto threads) {
     using T = decltype(t);
     using R = decltype(r);
-    block_norm_kernel<T, R, decltype(k)::value, decltype(multi)::value><<<dim3(grid), dim3(p.threads), 0, as_stream(stream)>>>(
+    block_norm_kernel<T, R, decltype(k)::value, decltype(form)::value, decltype(threads)::value><<<dim3(grid), dim3(p.threads), 0, as_stream(stream)>>>(
         a, (const T*)d_y, (const T*)d_gate, (const R*)d_residual, (R*)d_residual_out, residual_out_stride, (T*)d_normed, normed_stride);
     DC_LAUNCH_CHECK();
     return DC_OK;
@@ -476,11 +635,11 @@ extern "C" int dc_block_norm_backward(void* stream, int32_t dtype, int32_t resid
   const int groups = p.n_waves > 1 ? p.threads / 64 / p.n_waves : p.threads >> p.lane_bits;
   const int grid = parts_of(n_rows, width);
   const bool any = d_grad_scale || d_grad_post_w || d_grad_post_b || d_grad_pre_w || d_grad_pre_b;
-  return with_row(dtype, residual_dtype, p, [&](auto t, auto r, auto k, auto multi) {
+  return with_row(dtype, residual_dtype, p, [&](auto t, auto r, auto k, auto form, auto threads) {
     using T = decltype(t);
     using R = decltype(r);
     if (grid > 0) {
-      auto kernel = block_norm_backward_kernel<T, R, decltype(k)::value, decltype(multi)::value>;
+      auto kernel = block_norm_backward_kernel<T, R, decltype(k)::value, decltype(form)::value, decltype(threads)::value>;
       DC_SET_MAX_SMEM_ONCE_PER_DEVICE(kernel, DC_MAX_NORM_WIDTH * 4);
       kernel<<<dim3(grid), dim3(p.threads), groups * width * 4, as_stream(stream)>>>(
           a, (const T*)d_y, (const T*)d_gate, (const R*)d_residual, (const R*)d_grad_residual_out, grad_residual_out_stride,
