@@ -1,4 +1,18 @@
 // dc_token_logprobs: log probabilities of given tokens, entropy and top alternatives of rows of logits, and their gradient.
+//
+// HBM-bound: a row is read once (backward: read once, written once).  With m the row's maximum, S = sum exp(z - m) and
+// U = sum exp(z - m) (z - m):   log p_j = (z_j - m) - log S    H = log S - U / S    dz_j = p_j (-g - h (log p_j + H)) + g [j = t]
+//
+// Up to 512 classes a row lives in the registers of 1 to 64 lanes (4 neighbouring classes a lane; 8 beyond 256), forward and backward:
+// the two-class logits of a predict batch are one lane a row.  There S is summed without its largest term's 1 and log S = log1p(S - 1), so a
+// row that is sure of its class keeps the digits of -log p.
+// Beyond, a wavefront walks the row (or, where there are few rows, one of up to 64 slices of it, joined by a second kernel) in pieces of
+// 64 x 64 bytes kept in registers: running maximum, S and U per lane, joined at the end.
+// Top alternatives of a walk: the n-th largest of the lanes' (or quads') maxima bounds the n-th largest class from below, so one comparison
+// a class against that bound leaves a few candidates, which are collected in LDS and ranked by counting; the bound only rises from
+// there on.  Ties go to the lower class throughout: candidates are ordered by (logit, class).
+#include <type_traits>
+
 #include "elem_io.h"
 
 namespace dc {
@@ -19,116 +33,561 @@ __device__ __forceinline__ int64_t token_at(const Tokens& t, int64_t i) {
   }
 }
 
-// a float's place in ascending order as an unsigned number: -0 with +0, every NaN above +inf, none 0xffffffff
+// a float's place in ascending order as an unsigned number, never 0 or 0xffffffff: -0 with +0, every NaN above +inf
 __device__ __forceinline__ uint32_t order_key(float z) {
   if (!(z == z)) return 0xfffffffeu;
   const uint32_t u = __float_as_uint(z + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return k == 0xfffffffeu ? __builtin_nanf("") : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
 
 struct RowStats {
   float m, log_sum, entropy;  // max, log sum exp(z - m), entropy
 };
+__device__ __forceinline__ float log_prob(const RowStats& r, float z) { return r.m == -INFINITY ? -INFINITY : (z - r.m) - r.log_sum; }
 
-// One wavefront per row, three passes over it.
-template <typename T>
-__device__ RowStats row_stats(const T* z, int n) {
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-  bool bad = false;
-  for (int j = lane; j < n; j += 64) {
-    const float v = (float)z[j];
-    bad |= !(v == v) || v == INFINITY;
-    m = fmaxf(m, v);
-  }
+// dz without the given token's + g
+__device__ __forceinline__ float grad_at(const RowStats& r, float z, float g, float h) {
+  const float lp = (z - r.m) - r.log_sum, p = fast_exp2(lp * kLog2e);
+  return p == 0.0f ? 0.0f : -p * __builtin_fmaf(h, lp + r.entropy, g);
+}
+
+// what a row's gradient is: as the formula says, zeros (skipped, or nothing is possible), or NaN (a token outside the classes)
+enum RowGrad { kFormula, kZeros, kNans };
+__device__ __forceinline__ RowGrad row_grad(bool skip, const RowStats& r, bool wrong) {
+  return skip || r.m == -INFINITY ? kZeros : wrong ? kNans : kFormula;
+}
+
+template <typename Op>
+__device__ __forceinline__ uint32_t lanes_reduce_u32(uint32_t v, int bits, Op op) {
+  return __float_as_uint(lanes_reduce(__uint_as_float(v), bits, [&](float a, float b) { return __uint_as_float(op(__float_as_uint(a), __float_as_uint(b))); }));
+}
+
+// ---- up to 512 classes: a row in the registers of 2^bits lanes ------------------------------------------------------------------
+template <int E>
+struct Few {
+  static constexpr int W = E < 4 ? E : 4;  // neighbouring classes of a lane
+  float z[E];
+  int c[E];  // their class numbers
+};
+
+// -inf beyond the classes
+template <int E, typename T>
+__device__ __forceinline__ void load_few(const T* row, int n, int lane, int bits, Few<E>& f) {
+  constexpr int W = Few<E>::W;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-  if (__any(bad)) return {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-  if (m == -INFINITY) return {m, 0.0f, 0.0f};
-  // the sum without the largest term's 1, so that log S = log1p(...) keeps its digits where one class has all the weight
-  float s = 0.0f, u = 0.0f, ones = 0.0f;
-  for (int j = lane; j < n; j += 64) {
-    const float d = (float)z[j] - m, e = fast_exp2(d * kLog2e);
-    if (d == 0.0f) {
-      ones += 1.0f;
-    } else if (e > 0.0f) {
-      s += e;
-      u += e * d;
+  for (int k = 0; k < E / W; ++k) {
+    const int c = ((k << bits) + lane) * W;
+    float v[W];
+    if (c + W <= n) {
+      load_vec<W>(row + c, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) v[i] = c + i < n ? (float)row[c + i] : -INFINITY;
     }
+#pragma unroll
+    for (int i = 0; i < W; ++i) f.z[k * W + i] = v[i], f.c[k * W + i] = c + i;
   }
-  s = wave_sum(s) + (wave_sum(ones) - 1.0f);
-  u = wave_sum(u);
+}
+
+template <int E>
+__device__ __forceinline__ RowStats few_stats(const Few<E>& f, int bits) {
+  float m = f.z[0];
+#pragma unroll
+  for (int i = 1; i < E; ++i) m = __builtin_fmaxf(m, f.z[i]);
+  m = lanes_max(m, bits);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float s = 0.0f, u = 0.0f, ones = 0.0f;  // (a NaN, or the NaN of inf - inf, reaches s and all that comes of it)
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const float d = f.z[i] - ref, e = fast_exp2(d * kLog2e);
+    ones += d == 0.0f ? 1.0f : 0.0f;
+    s += d == 0.0f ? 0.0f : e;
+    u += e > 0.0f ? e * d : 0.0f;
+  }
+  s = lanes_sum(s, bits);
+  ones = lanes_sum(ones, bits);
+  u = lanes_sum(u, bits);
+  if (m == -INFINITY && s == 0.0f) return {m, 0.0f, 0.0f};
+  s += ones - 1.0f;
   const float log_sum = log1pf(s);
-  return {m, log_sum, log_sum - u / (1.0f + s)};
+  return {ref, log_sum, log_sum - u * fast_rcp(1.0f + s)};
 }
 
-__device__ __forceinline__ float log_prob(const RowStats& r, float z) {
-  return r.m == -INFINITY ? -INFINITY : (z - r.m) - r.log_sum;
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void token_logprobs_kernel(const T* __restrict__ logits, int64_t n_rows, int32_t n, int64_t ld, Tokens tok, int32_t n_top,
-                                                             float* logprob, float* entropy, float* stats, int32_t* top_ids, float* top_logprob) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n_rows; i += (int64_t)gridDim.x * 4) {
+template <typename T, int E>
+__global__ __launch_bounds__(256) void few_classes_kernel(const T* __restrict__ logits, int64_t n_rows, int32_t n, int64_t ld, int32_t bits, Tokens tok,
+                                                          int32_t n_top, float* __restrict__ logprob, float* __restrict__ entropy,
+                                                          float* __restrict__ stats, int32_t* __restrict__ top_ids, float* __restrict__ top_logprob) {
+  const int lane = threadIdx.x & ((1 << bits) - 1);
+  const int64_t step = (int64_t)gridDim.x * (256 >> bits);
+  for (int64_t i = (int64_t)blockIdx.x * (256 >> bits) + (threadIdx.x >> bits); i < n_rows; i += step) {
     const int64_t t = tok.p ? token_at(tok, i) : 0;
     const bool skip = tok.p && t == tok.ignore;
-    const T* z = logits + i * ld;
     RowStats r{0.0f, 0.0f, 0.0f};
-    if (!skip) r = row_stats(z, n);
+    Few<E> f;
+    if (!skip) {
+      load_few<E>(logits + i * ld, n, lane, bits, f);
+      r = few_stats<E>(f, bits);
+    }
+    if (logprob && tok.p) {
+      float lp = 0.0f;
+      if (!skip) {
+        lp = __builtin_nanf("");
+        bool mine = lane == 0 && !(t >= 0 && t < n);  // the lane that holds the token's class, or the first one for a wrong token
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+          if (f.c[k] == t && t < n) lp = log_prob(r, f.z[k]), mine = true;
+        if (mine) logprob[i] = lp;
+      } else if (lane == 0) {
+        logprob[i] = lp;
+      }
+    }
     if (lane == 0) {
-      if (logprob && tok.p) logprob[i] = skip ? 0.0f : t >= 0 && t < n ? log_prob(r, (float)z[t]) : __builtin_nanf("");
       if (entropy) entropy[i] = r.entropy;
       if (stats) stats[3 * i] = r.m, stats[3 * i + 1] = r.log_sum, stats[3 * i + 2] = r.entropy;
     }
-    uint64_t below = ~0ull;  // (key, ~class) of the alternative found last
+    uint32_t used = 0;
     for (int k = 0; k < n_top; ++k) {
-      uint64_t best = 0;
+      float lp = 0.0f;
+      int id = -1;
       if (!skip) {
-        for (int j = lane; j < n; j += 64) {
-          const uint64_t c = (uint64_t)order_key((float)z[j]) << 32 | (uint32_t)~j;
-          if (c < below && c > best) best = c;
-        }
+        uint32_t key = 0;
+        int at = 0;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const uint64_t o = __shfl_xor(best, d, 64);
-          if (o > best) best = o;
+        for (int q = 0; q < E; ++q) {
+          const uint32_t o = f.c[q] < n && !(used >> q & 1) ? order_key(f.z[q]) : 0;
+          if (o > key) key = o, at = q;
         }
+        const uint32_t best = lanes_reduce_u32(key, bits, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        int c = 0;
+#pragma unroll
+        for (int q = 0; q < E; ++q)
+          if (q == at) c = f.c[q];
+        id = (int)lanes_reduce_u32(key == best ? (uint32_t)c : 0x7fffffffu, bits, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+        if (key == best && c == id) used |= 1u << at;
+        lp = log_prob(r, key_value(best));
       }
-      below = best;
-      if (lane == 0) {
-        const int id = skip ? -1 : (int)~(uint32_t)best;
-        top_ids[i * n_top + k] = id;
-        top_logprob[i * n_top + k] = skip ? 0.0f : log_prob(r, (float)z[id]);
+      if (lane == 0) top_ids[i * n_top + k] = id, top_logprob[i * n_top + k] = lp;
+    }
+  }
+}
+
+template <typename T, int E>
+__global__ __launch_bounds__(256) void few_classes_backward_kernel(const T* logits, int64_t n_rows, int32_t n, int64_t ld, int32_t bits, Tokens tok,
+                                                                   const float* __restrict__ g_logprob, const float* __restrict__ g_entropy, T* out,
+                                                                   int64_t ld_out) {
+  constexpr int W = Few<E>::W;
+  const int lane = threadIdx.x & ((1 << bits) - 1);
+  const int64_t step = (int64_t)gridDim.x * (256 >> bits);
+  for (int64_t i = (int64_t)blockIdx.x * (256 >> bits) + (threadIdx.x >> bits); i < n_rows; i += step) {
+    const int64_t t = tok.p ? token_at(tok, i) : -1;
+    const bool skip = tok.p && t == tok.ignore;
+    RowStats r{-INFINITY, 0.0f, 0.0f};
+    Few<E> f;
+    float g = 0.0f, h = 0.0f;
+    if (!skip) {
+      g = g_logprob ? g_logprob[i] : 0.0f, h = g_entropy ? g_entropy[i] : 0.0f;
+      load_few<E>(logits + i * ld, n, lane, bits, f);
+      r = few_stats<E>(f, bits);
+    }
+    const RowGrad what = row_grad(skip, r, g_logprob && !(t >= 0 && t < n));
+#pragma unroll
+    for (int k = 0; k < E / W; ++k) {
+      const int c = ((k << bits) + lane) * W;
+      float v[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        v[w] = what == kZeros ? 0.0f : what == kNans ? __builtin_nanf("") : grad_at(r, f.z[k * W + w], g, h);
+        if (what == kFormula && c + w == t) v[w] += g;
+      }
+      T* o = out + i * ld_out + c;
+      if (c + W <= n) {
+        store_vec<W>(o, v);
+      } else {
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          if (c + w < n) o[w] = (T)v[w];
       }
     }
   }
 }
 
+// ---- more classes: a wavefront walks a row or a slice of it ---------------------------------------------------------------------
+constexpr int kVectors = 4;  // 16-byte vectors of a lane in a piece
+constexpr int kMaxSlices = 64;
+
+// A row in aligned 16-byte vectors and what is left at its two ends.
 template <typename T>
-__global__ __launch_bounds__(256) void token_logprobs_backward_kernel(const T* logits, int64_t n_rows, int32_t n, int64_t ld, Tokens tok,
-                                                                      const float* stats, const float* g_logprob, const float* g_entropy, T* out,
-                                                                      int64_t ld_out) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < n_rows; i += (int64_t)gridDim.x * 4) {
-    const int64_t t = tok.p ? token_at(tok, i) : -1;
-    const bool skip = tok.p && t == tok.ignore;
-    const T* z = logits + i * ld;
-    RowStats r{0.0f, 0.0f, 0.0f};
-    if (!skip) r = stats ? RowStats{stats[3 * i], stats[3 * i + 1], stats[3 * i + 2]} : row_stats(z, n);
-    const float g = g_logprob ? g_logprob[i] : 0.0f, h = g_entropy ? g_entropy[i] : 0.0f;
-    const bool wrong = g_logprob && !(t >= 0 && t < n);
-    for (int j = lane; j < n; j += 64) {
-      float d = 0.0f;
-      if (!skip && r.m != -INFINITY) {
-        const float lp = log_prob(r, (float)z[j]), p = fast_exp2(lp * kLog2e);
-        d = p > 0.0f || p != p ? -p * (g + h * (lp + r.entropy)) : 0.0f;
-        if (j == t) d += g;
-        if (wrong) d = __builtin_nanf("");
-      }
-      out[i * ld_out + j] = (T)d;
+struct Layout {
+  static constexpr int W = 16 / sizeof(T);
+  int head, n_vec, tail;
+  __device__ __forceinline__ Layout(const T* row, int n) {
+    head = (int)((-(reinterpret_cast<uintptr_t>(row) / sizeof(T))) & (W - 1));
+    if (head > n) head = n;
+    n_vec = (n - head) / W;
+    tail = n - head - n_vec * W;
+  }
+};
+
+// max, S and U about it (U in powers of two); m = -inf, S = 0: nothing yet
+struct Running {
+  float m, s, u;
+};
+__device__ __forceinline__ Running merged(const Running& a, const Running& b) {
+  const float m = __builtin_fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.0f : m;
+  Running r{m, 0.0f, 0.0f};
+  for (const Running& x : {a, b}) {
+    // (S of a part that has seen only -inf is 0, or NaN; below 2^-200 a part counts for nothing, and 0 x -inf is not wanted)
+    const float d = x.m == -INFINITY ? 0.0f : __builtin_fmaxf((x.m - ref) * kLog2e, -200.0f);
+    const float f = fast_exp2(d);
+    r.s = __builtin_fmaf(f, x.s, r.s);
+    r.u = __builtin_fmaf(f, __builtin_fmaf(d, x.s, x.u), r.u);
+  }
+  return r;
+}
+__device__ __forceinline__ Running wave_merged(Running r) {
+  const float m = lanes_max(r.m, 6), ref = m == -INFINITY ? 0.0f : m;
+  const float d = r.m == -INFINITY ? 0.0f : __builtin_fmaxf((r.m - ref) * kLog2e, -200.0f), f = fast_exp2(d);
+  return {m, wave_sum(f * r.s), wave_sum(f * __builtin_fmaf(d, r.s, r.u))};
+}
+__device__ __forceinline__ RowStats finish(const Running& r) {
+  if (r.m == -INFINITY && r.s == 0.0f) return {r.m, 0.0f, 0.0f};
+  const float log_sum = logf(r.s);
+  return {r.m == -INFINITY ? 0.0f : r.m, log_sum, log_sum - kLn2 * r.u / r.s};
+}
+
+// Candidates of one wavefront in LDS: (key, ~class) as one number, larger is better.
+struct Candidates {
+  uint64_t* list;  // [128]
+  int n, k;        // collected, wanted
+  float bound;     // a class below it is none of the k best
+  uint64_t worst;  // the k-th best of those ranked so far, or 0
+
+  __device__ __forceinline__ void start(uint64_t* lds, int wanted) { list = lds, n = 0, k = wanted, bound = -INFINITY, worst = 0; }
+
+  // the lanes of `has` add theirs; a full list is ranked first
+  __device__ __forceinline__ void add(bool has, uint64_t cand) {
+    uint64_t mask = __ballot(has && cand > worst);
+    if (!mask) return;
+    if (n > 64) {
+      rank();
+      mask = __ballot(has && cand > worst);
+    }
+    if (mask >> (threadIdx.x & 63) & 1) list[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = cand;
+    n += __popcll(mask);
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // the k best, in order, to the front of the list: everyone counts how many are better than its one or two
+  __device__ void rank() {
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_wave_barrier();
+    const uint64_t a = lane < n ? list[lane] : 0, b = lane + 64 < n ? list[lane + 64] : 0;
+    int ra = 0, rb = 0;
+    for (int i = 0; i < n; ++i) {
+      const uint64_t o = list[i];
+      ra += o > a, rb += o > b;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (lane < n && ra < k) list[ra] = a;
+    if (lane + 64 < n && rb < k) list[rb] = b;
+    __builtin_amdgcn_wave_barrier();
+    if (n >= k) {
+      n = k;
+      worst = list[k - 1];
+      const float v = key_value((uint32_t)(worst >> 32));
+      bound = v;  // (a NaN bound lets every class through to the comparison with `worst`)
     }
   }
+};
+__device__ __forceinline__ uint64_t candidate(float z, int c) { return (uint64_t)order_key(z) << 32 | (uint32_t)~c; }
+
+// The k-th largest of the maxima of 64 lanes, or of 16 quads where that is enough: at least k classes are no smaller.
+__device__ __forceinline__ float first_bound(float lane_max, int k) {
+  int rank = 0;
+  const int lane = threadIdx.x & 63;
+  if (k <= 8) {
+    const float q = lanes_max(lane_max, 2);
+    for (int i = 0; i < 64; i += 4) {
+      const float o = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(q), i));
+      rank += o > q || (o == q && i < (lane & ~3));
+    }
+    lane_max = q;
+    const uint64_t hit = __ballot(rank == k - 1);
+    return hit ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lane_max), __builtin_ctzll(hit))) : -INFINITY;
+  }
+  for (int i = 0; i < 64; ++i) {
+    const float o = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lane_max), i));
+    rank += o > lane_max || (o == lane_max && i < lane);
+  }
+  const uint64_t hit = __ballot(rank == k - 1);
+  return hit ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lane_max), __builtin_ctzll(hit))) : -INFINITY;
+}
+
+// What a slice leaves for the join: m, S, U and its k best candidates.
+struct Slices {
+  int32_t n;        // of a row; 1: no join
+  float* running;   // [row][slice][3]
+  uint64_t* best;   // [row][slice][n_top]
+};
+
+struct ManyOut {
+  float *logprob, *entropy, *stats;
+  int32_t* top_ids;
+  float* top_logprob;
+};
+
+// one row's results, by the lanes of one wavefront
+template <typename T>
+__device__ __forceinline__ void write_row(const ManyOut& out, int64_t i, const T* row, int n, int64_t t, bool have_token, const RowStats& r, int n_top,
+                                          const uint64_t* best) {
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) {
+    if (out.logprob && have_token) out.logprob[i] = t >= 0 && t < n ? log_prob(r, (float)row[t]) : __builtin_nanf("");
+    if (out.entropy) out.entropy[i] = r.entropy;
+    if (out.stats) out.stats[3 * i] = r.m, out.stats[3 * i + 1] = r.log_sum, out.stats[3 * i + 2] = r.entropy;
+  }
+  if (lane < n_top) {
+    out.top_ids[i * n_top + lane] = (int)~(uint32_t)best[lane];
+    out.top_logprob[i * n_top + lane] = log_prob(r, key_value((uint32_t)(best[lane] >> 32)));
+  }
+}
+__device__ __forceinline__ void write_skipped(const ManyOut& out, int64_t i, int n_top) {
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) {
+    if (out.logprob) out.logprob[i] = 0.0f;
+    if (out.entropy) out.entropy[i] = 0.0f;
+    if (out.stats) out.stats[3 * i] = out.stats[3 * i + 1] = out.stats[3 * i + 2] = 0.0f;
+  }
+  if (lane < n_top) out.top_ids[i * n_top + lane] = -1, out.top_logprob[i * n_top + lane] = 0.0f;
+}
+
+template <typename T, bool TOP>
+__global__ __launch_bounds__(256) void many_classes_kernel(const T* __restrict__ logits, int64_t n_rows, int32_t n, int64_t ld, Tokens tok, int32_t n_top,
+                                                           Slices sl, ManyOut out) {
+  constexpr int W = 16 / sizeof(T);
+  using Vec = vec_t<T, W>;
+  __shared__ uint64_t lds[4][128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n_units = n_rows * sl.n;
+  for (int64_t unit = (int64_t)blockIdx.x * 4 + wave; unit < n_units; unit += (int64_t)gridDim.x * 4) {
+    const int64_t i = unit / sl.n;
+    const int slice = (int)(unit - i * sl.n);
+    const int64_t t = tok.p ? token_at(tok, i) : 0;
+    if (tok.p && t == tok.ignore) {
+      if (sl.n == 1) write_skipped(out, i, n_top);
+      continue;
+    }
+    const T* row = logits + i * ld;
+    const Layout<T> at(row, n);
+    const Vec* vecs = reinterpret_cast<const Vec*>(row + at.head);
+    const int v0 = (int)((int64_t)at.n_vec * slice / sl.n), v1 = (int)((int64_t)at.n_vec * (slice + 1) / sl.n);
+    // the row's ends, a class a lane: the head with the first slice (its classes come first), the tail with the last (last)
+    const bool head = slice == 0 && lane < at.head, tail = slice == sl.n - 1 && lane < at.tail;
+    const int tail_c = at.head + at.n_vec * W + lane;
+    const float z_head = head ? (float)row[lane] : -INFINITY, z_tail = tail ? (float)row[tail_c] : -INFINITY;
+    Vec raw[kVectors];
+    auto fetch = [&](int v) {
+#pragma unroll
+      for (int q = 0; q < kVectors; ++q)
+        if (v + q * 64 + lane < v1) raw[q] = vecs[v + q * 64 + lane];
+    };
+    fetch(v0);
+    Running r{-INFINITY, 0.0f, 0.0f};
+    auto take = [&](float z) {  // a class of the row's ends
+      const bool any = z != -INFINITY;
+      r = merged(r, Running{z, any ? (z - z == 0.0f ? 1.0f : __builtin_nanf("")) : 0.0f, 0.0f});
+    };
+    take(z_head);
+    take(z_tail);
+    Candidates best;
+    if constexpr (TOP) {
+      best.start(lds[wave], n_top);
+    }
+    for (int v = v0; v < v1; v += 64 * kVectors) {
+      float z[kVectors][W];
+#pragma unroll
+      for (int q = 0; q < kVectors; ++q) {
+        const bool in = v + q * 64 + lane < v1;
+#pragma unroll
+        for (int w = 0; w < W; ++w) z[q][w] = in ? (float)raw[q][w] : -INFINITY;
+      }
+      if (v + 64 * kVectors < v1) fetch(v + 64 * kVectors);
+      float pm = z[0][0];
+#pragma unroll
+      for (int q = 0; q < kVectors; ++q)
+#pragma unroll
+        for (int w = 0; w < W; ++w) pm = __builtin_fmaxf(pm, z[q][w]);
+      if (!(pm <= r.m)) {  // the lane's maximum moves
+        const float ref = pm == -INFINITY ? 0.0f : pm, d = r.m == -INFINITY ? 0.0f : __builtin_fmaxf((r.m - ref) * kLog2e, -200.0f), f = fast_exp2(d);
+        r.u = f * __builtin_fmaf(d, r.s, r.u);
+        r.s *= f;
+        r.m = __builtin_fmaxf(pm, r.m);
+      }
+      const float ref = r.m == -INFINITY ? 0.0f : r.m;
+#pragma unroll
+      for (int q = 0; q < kVectors; ++q) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float d = (z[q][w] - ref) * kLog2e, e = fast_exp2(d);
+          r.s += e;
+          r.u = __builtin_fmaf(e, __builtin_fmaxf(d, -200.0f), r.u);  // (e is 0 there, and 0 x -inf is not wanted)
+        }
+      }
+      if constexpr (TOP) {
+        if (v == v0) {
+          best.bound = first_bound(pm, n_top);
+          best.add(head, candidate(z_head, lane));
+        }
+#pragma unroll
+        for (int q = 0; q < kVectors; ++q) {
+          const bool in = v + q * 64 + lane < v1;
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            const bool may = in && !(z[q][w] < best.bound);
+            if (__ballot(may)) best.add(may, candidate(z[q][w], at.head + (v + q * 64 + lane) * W + w));
+          }
+        }
+        if (v == v0) best.rank();
+      }
+    }
+    if constexpr (TOP) {
+      if (v0 >= v1) best.add(head, candidate(z_head, lane));
+      best.add(tail, candidate(z_tail, tail_c));
+      best.rank();
+    }
+    r = wave_merged(r);
+    if (sl.n == 1) {
+      write_row(out, i, row, n, t, tok.p != nullptr, finish(r), TOP ? n_top : 0, lds[wave]);
+    } else {
+      if (lane == 0) {
+        float* p = sl.running + unit * 3;
+        p[0] = r.m, p[1] = r.s, p[2] = r.u;
+      }
+      if constexpr (TOP) {
+        if (lane < n_top) sl.best[unit * n_top + lane] = lane < best.n ? best.list[lane] : 0;
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The slices of a row, by one wavefront: a lane holds a slice's sums.
+template <typename T>
+__global__ __launch_bounds__(64) void join_slices_kernel(const T* __restrict__ logits, int64_t n_rows, int32_t n, int64_t ld, Tokens tok, int32_t n_top,
+                                                         Slices sl, ManyOut out) {
+  __shared__ uint64_t lds[128];
+  const int lane = threadIdx.x;
+  for (int64_t i = blockIdx.x; i < n_rows; i += gridDim.x) {
+    const int64_t t = tok.p ? token_at(tok, i) : 0;
+    if (tok.p && t == tok.ignore) {
+      write_skipped(out, i, n_top);
+      continue;
+    }
+    Running r{-INFINITY, 0.0f, 0.0f};
+    if (lane < sl.n) {
+      const float* p = sl.running + (i * sl.n + lane) * 3;
+      r = {p[0], p[1], p[2]};
+    }
+    r = wave_merged(r);
+    Candidates best;
+    if (n_top > 0) {
+      best.start(lds, n_top);
+      const uint64_t* from = sl.best + i * sl.n * n_top;
+      const uint64_t top = lane < sl.n ? from[lane * n_top] : 0;  // (0: no candidate)
+      const float b = first_bound(top ? key_value((uint32_t)(top >> 32)) : -INFINITY, n_top);
+      for (int c = 0; c < sl.n * n_top; c += 64) {
+        const uint64_t cand = c + lane < sl.n * n_top ? from[c + lane] : 0;
+        const bool may = cand != 0 && !(key_value((uint32_t)(cand >> 32)) < b);
+        if (__ballot(may)) best.add(may, cand);
+      }
+      best.rank();
+    }
+    write_row(out, i, logits + i * ld, n, t, tok.p != nullptr, finish(r), n_top, lds);
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// A workgroup per kVectors x 256 vectors of a row; the first one also takes the row's head, the last its tail.
+template <typename T>
+__global__ __launch_bounds__(256) void many_classes_backward_kernel(const T* logits, int64_t n_rows, int32_t n, int64_t ld, Tokens tok,
+                                                                    const float* __restrict__ stats, const float* __restrict__ g_logprob,
+                                                                    const float* __restrict__ g_entropy, T* out, int64_t ld_out, int32_t n_blocks) {
+  constexpr int W = 16 / sizeof(T);
+  using Vec = vec_t<T, W>;
+  for (int64_t unit = blockIdx.x; unit < n_rows * n_blocks; unit += gridDim.x) {
+    const int64_t i = unit / n_blocks;
+    const int b = (int)(unit - i * n_blocks);
+    const T* row = logits + i * ld;
+    T* o = out + i * ld_out;
+    const Layout<T> at(row, n);
+    const Vec* vecs = reinterpret_cast<const Vec*>(row + at.head);
+    const int v0 = b * kVectors * 256 + threadIdx.x;
+    Vec raw[kVectors];
+    const int64_t t = tok.p ? token_at(tok, i) : -1;
+    const bool skip = tok.p && t == tok.ignore;
+    if (!skip) {
+#pragma unroll
+      for (int q = 0; q < kVectors; ++q)
+        if (v0 + q * 256 < at.n_vec) raw[q] = vecs[v0 + q * 256];
+    }
+    const RowStats r{stats[3 * i], stats[3 * i + 1], stats[3 * i + 2]};
+    const float g = g_logprob ? g_logprob[i] : 0.0f, h = g_entropy ? g_entropy[i] : 0.0f;
+    const RowGrad what = row_grad(skip, r, g_logprob && !(t >= 0 && t < n));
+    const float flat = what == kNans ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+    for (int q = 0; q < kVectors; ++q) {
+      const int v = v0 + q * 256;
+      if (v >= at.n_vec) continue;
+      const int c = at.head + v * W;
+      float d[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) d[w] = flat;
+      if (what == kFormula) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) d[w] = grad_at(r, (float)raw[q][w], g, h);
+        if (t >= c && t < c + W) {
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            if (c + w == t) d[w] += g;
+        }
+      }
+      store_vec<W>(o + c, d);
+    }
+    const int tail_at = at.head + at.n_vec * W;
+    const bool first = b == 0 && (int)threadIdx.x < at.head, last = b == n_blocks - 1 && (int)threadIdx.x < at.tail;
+    for (int e = 0; e < 2; ++e) {
+      if (!(e ? last : first)) continue;
+      const int c = (e ? tail_at : 0) + threadIdx.x;
+      o[c] = (T)(what == kFormula ? grad_at(r, (float)row[c], g, h) + (c == t ? g : 0.0f) : flat);
+    }
+  }
+}
+
+// How a forward call is divided beyond DC_STATS_FROM classes: about four wavefronts a SIMD, slices of at least 1 024 classes.
+int slices_of(int64_t n_rows, int32_t n_classes) {
+  if (n_rows <= 0 || n_rows >= 2048 || n_classes < DC_STATS_FROM) return 1;
+  int64_t s = (4096 + n_rows - 1) / n_rows;
+  if (s > n_classes / 1024) s = n_classes / 1024;
+  return (int)(s > kMaxSlices ? kMaxSlices : s < 1 ? 1 : s);
+}
+
+// lanes a row takes up to 512 classes, as a power of two
+int lane_bits_of(int32_t n_classes) {
+  int bits = 0;
+  while (n_classes > 4 << bits && bits < 6) ++bits;
+  return bits;
+}
+
+// calls f with the element type and the classes a lane
+template <typename F>
+int with_few(int32_t dtype, int32_t n_classes, F&& f) {
+  return with_dtype(dtype, [&](auto t) {
+    if (n_classes <= 2) return f(t, std::integral_constant<int, 2>{});
+    return n_classes <= 256 ? f(t, std::integral_constant<int, 4>{}) : f(t, std::integral_constant<int, 8>{});
+  });
 }
 
 int check_logits(const void* logits, int32_t dtype, int64_t n_rows, int32_t n_classes, int64_t row_stride, const void* tokens, int32_t token_type) {
@@ -142,15 +601,15 @@ int check_logits(const void* logits, int32_t dtype, int64_t n_rows, int32_t n_cl
   return DC_OK;
 }
 
-unsigned row_grid(int64_t n_rows) {
-  const int64_t b = (n_rows + 3) / 4;
-  return (unsigned)(b < (1 << 20) ? b : 1 << 20);
-}
+unsigned grid_of(int64_t blocks) { return (unsigned)(blocks < (1 << 22) ? blocks : 1 << 22); }
 
 }  // namespace
 }  // namespace dc
 
-extern "C" int64_t dc_token_logprobs_workspace(int64_t, int32_t, int32_t) { return 0; }
+extern "C" int64_t dc_token_logprobs_workspace(int64_t n_rows, int32_t n_classes, int32_t n_top) {
+  const int64_t s = dc::slices_of(n_rows, n_classes);
+  return s > 1 ? n_rows * s * ((n_top > 0 ? n_top : 0) * 8 + 12) : 0;
+}
 
 extern "C" int dc_token_logprobs(void* stream, const void* d_logits, int32_t dtype, int64_t n_rows, int32_t n_classes, int64_t row_stride,
                                  const void* d_tokens, int32_t token_type, int64_t ignore_token, int32_t n_top, float* d_logprob, float* d_entropy,
@@ -159,14 +618,34 @@ extern "C" int dc_token_logprobs(void* stream, const void* d_logits, int32_t dty
   if (int rc = check_logits(d_logits, dtype, n_rows, n_classes, row_stride, d_tokens, token_type)) return rc;
   DC_REQUIRE(n_top >= 0 && n_top <= n_classes && n_top <= DC_MAX_TOP, "n_top must be in [0, min(n_classes, 32)]");
   DC_REQUIRE(n_rows == 0 || n_top == 0 || (d_top_ids && d_top_logprob), "null pointer");
-  (void)d_workspace, (void)workspace_bytes;
+  const int64_t need = dc_token_logprobs_workspace(n_rows, n_classes, n_top);
+  DC_REQUIRE(workspace_bytes >= need && (need == 0 || d_workspace) && aligned(d_workspace, 16), "workspace too small");
   if (n_rows == 0) return DC_OK;
+  const Tokens tok{d_tokens, token_type, ignore_token};
+  if (n_classes < DC_STATS_FROM) {
+    const int bits = lane_bits_of(n_classes);
+    return with_few(dtype, n_classes, [&](auto t, auto e) {
+      using T = decltype(t);
+      few_classes_kernel<T, decltype(e)::value><<<dim3(grid_of((n_rows + (256 >> bits) - 1) / (256 >> bits))), dim3(256), 0, as_stream(stream)>>>(
+          (const T*)d_logits, n_rows, n_classes, row_stride, bits, tok, n_top, d_logprob, d_entropy, d_stats, d_top_ids, d_top_logprob);
+      DC_LAUNCH_CHECK();
+      return DC_OK;
+    });
+  }
+  const int s = slices_of(n_rows, n_classes);
+  uint64_t* best = (uint64_t*)d_workspace;
+  const Slices sl{s, (float*)(best + (s > 1 ? n_rows * s * n_top : 0)), best};
+  const ManyOut out{d_logprob, d_entropy, d_stats, d_top_ids, d_top_logprob};
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    token_logprobs_kernel<T><<<dim3(row_grid(n_rows)), dim3(256), 0, as_stream(stream)>>>((const T*)d_logits, n_rows, n_classes, row_stride,
-                                                                                          Tokens{d_tokens, token_type, ignore_token}, n_top, d_logprob,
-                                                                                          d_entropy, d_stats, d_top_ids, d_top_logprob);
+    const dim3 grid(grid_of((n_rows * s + 3) / 4));
+    if (n_top > 0) many_classes_kernel<T, true><<<grid, dim3(256), 0, as_stream(stream)>>>((const T*)d_logits, n_rows, n_classes, row_stride, tok, n_top, sl, out);
+    else many_classes_kernel<T, false><<<grid, dim3(256), 0, as_stream(stream)>>>((const T*)d_logits, n_rows, n_classes, row_stride, tok, n_top, sl, out);
     DC_LAUNCH_CHECK();
+    if (s > 1) {
+      join_slices_kernel<T><<<dim3(grid_of(n_rows)), dim3(64), 0, as_stream(stream)>>>((const T*)d_logits, n_rows, n_classes, row_stride, tok, n_top, sl, out);
+      DC_LAUNCH_CHECK();
+    }
     return DC_OK;
   });
 }
@@ -182,11 +661,22 @@ extern "C" int dc_token_logprobs_backward(void* stream, const void* d_logits, in
   DC_REQUIRE(grad_stride >= n_classes, "rows of the output overlap");
   DC_REQUIRE(aligned(d_grad_logits, dtype_size(dtype)), "misaligned pointer");
   if (n_rows == 0) return DC_OK;
+  const Tokens tok{d_tokens, token_type, ignore_token};
+  if (n_classes < DC_STATS_FROM) {
+    const int bits = lane_bits_of(n_classes);
+    return with_few(dtype, n_classes, [&](auto t, auto e) {
+      using T = decltype(t);
+      few_classes_backward_kernel<T, decltype(e)::value><<<dim3(grid_of((n_rows + (256 >> bits) - 1) / (256 >> bits))), dim3(256), 0, as_stream(stream)>>>(
+          (const T*)d_logits, n_rows, n_classes, row_stride, bits, tok, d_grad_logprob, d_grad_entropy, (T*)d_grad_logits, grad_stride);
+      DC_LAUNCH_CHECK();
+      return DC_OK;
+    });
+  }
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    token_logprobs_backward_kernel<T><<<dim3(row_grid(n_rows)), dim3(256), 0, as_stream(stream)>>>(
-        (const T*)d_logits, n_rows, n_classes, row_stride, Tokens{d_tokens, token_type, ignore_token}, d_stats, d_grad_logprob, d_grad_entropy,
-        (T*)d_grad_logits, grad_stride);
+    const int per_block = kVectors * 256 * (16 / (int)sizeof(T)), n_blocks = (n_classes + per_block - 1) / per_block;
+    many_classes_backward_kernel<T><<<dim3(grid_of(n_rows * n_blocks)), dim3(256), 0, as_stream(stream)>>>(
+        (const T*)d_logits, n_rows, n_classes, row_stride, tok, d_stats, d_grad_logprob, d_grad_entropy, (T*)d_grad_logits, grad_stride, n_blocks);
     DC_LAUNCH_CHECK();
     return DC_OK;
   });
