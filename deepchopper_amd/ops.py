@@ -199,12 +199,24 @@ _NORM_KINDS = {"layer": 0, "rms": 1}
 _GATE_ACTS = {"identity": 0, "sigmoid": 1, "silu": 2}
 STATS_FROM = 513  # DC_STATS_FROM: classes from which token_logprobs_backward needs the forward's statistics
 _NO_SWITCH = contextlib.nullcontext()
+try:  # (plain integers, a tenth of the cost of the objects torch.cuda makes of them: a step of a few tokens is as long as its call)
+    from torch._C import _cuda_getCurrentRawStream as _stream_of, _cuda_getDevice as _current_device
+except ImportError:
+    def _stream_of(dev: int) -> int:
+        return torch.cuda.current_stream(dev).cuda_stream
+
+    _current_device = torch.cuda.current_device
 
 
-def _on(t: torch.Tensor):
-    """Context in which `t`'s device is the current one (a call's kernels run on ITS device's current stream)."""
-    i = t.device.index
-    return _NO_SWITCH if i == torch.cuda.current_device() else torch.cuda.device(i)
+def _device_of(name: str, t: torch.Tensor) -> int:
+    if not t.is_cuda:
+        raise ValueError(f"{name}: device-resident tensor required, got one on {t.device}")
+    return t.get_device()
+
+
+def _on(dev: int):
+    """Context in which device `dev` is the current one (a call's kernels run on ITS tensors' device, on that device's current stream)."""
+    return _NO_SWITCH if dev == _current_device() else torch.cuda.device(dev)
 
 
 def _need(ok: bool, what: str) -> None:
@@ -212,32 +224,49 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _like(ref: torch.Tensor, name: str, t: torch.Tensor | None, shape, dtype: torch.dtype) -> int | None:
+def _like(dev: int, name: str, t: torch.Tensor | None, shape: tuple, dtype: torch.dtype) -> int | None:
     """Address of the contiguous tensor `t` (or None) after checking it against what the call needs."""
     if t is None:
         return None
-    _need(t.device == ref.device and t.dtype == dtype and t.shape == tuple(shape) and t.is_contiguous(),
-          f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on {ref.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.get_device() != dev or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{dev}, got {t.dtype} {tuple(t.shape)} "
+                         f"with strides {t.stride()} on {t.device}")
     return t.data_ptr()
 
 
-def _rows(ref: torch.Tensor, name: str, t: torch.Tensor | None, shape=None, dtype: torch.dtype | None = None) -> tuple[int | None, int]:
+def _rows(dev: int, name: str, t: torch.Tensor | None, shape: torch.Size | None = None, dtype: torch.dtype | None = None) -> tuple[int | None, int]:
     """(address, elements between rows) of a [..., width] tensor whose rows are contiguous and evenly spaced (the halves of
-    a projection, an expanded row), after checking it against `ref`'s device and the shape and type the call needs."""
+    a projection, an expanded row), after checking it against the device, shape and type the call needs."""
     if t is None:
         return None, 0
-    _need(t.is_cuda and t.device == ref.device, f"{name}: device-resident tensor on {ref.device} required, got {t.device}")
-    _need(shape is None or t.shape == shape, f"{name}: expected shape {tuple(shape or ())}, got {tuple(t.shape)}")
-    _need(t.dtype == dtype if dtype is not None else t.dtype in _DTYPES, f"{name}: {t.dtype} is not {dtype or 'float32, float16 or bfloat16'}")
-    _need(t.dim() >= 2, f"{name}: at least two dimensions required, got {t.dim()}")
-    size, st = t.shape, t.stride()
-    _need(st[-1] == 1 or size[-1] <= 1 or t.numel() == 0, f"{name}: the last dimension must be contiguous")
+    size = t.shape
+    if t.get_device() != dev or (shape is not None and size != shape) or (t.dtype is not dtype if dtype is not None else t.dtype not in _DTYPES) or len(size) < 2:
+        raise ValueError(f"{name}: expected {dtype or 'float32, float16 or bfloat16'} of shape {tuple(shape) if shape is not None else '[..., width]'} "
+                         f"on cuda:{dev}, got {t.dtype} {tuple(size)} on {t.device}")
+    if t.is_contiguous():
+        return t.data_ptr(), size[-1]
+    st = t.stride()
+    if st[-1] != 1 and size[-1] > 1 and t.numel():
+        raise ValueError(f"{name}: the last dimension must be contiguous (shape {tuple(size)}, strides {st})")
     # leading dimensions of size 1 say nothing about the distance of two rows
-    dims = [(n, s) for n, s in zip(size[:-1], st[:-1]) if n != 1]
-    if t.numel():
-        for (_, outer), (n, s) in zip(dims, dims[1:]):
-            _need(outer == n * s, f"{name}: rows must be evenly spaced (shape {tuple(size)}, strides {st})")
+    dims = [(n, d) for n, d in zip(size[:-1], st[:-1]) if n != 1]
+    for (_, outer), (n, d) in zip(dims, dims[1:]):
+        if outer != n * d and t.numel():
+            raise ValueError(f"{name}: rows must be evenly spaced (shape {tuple(size)}, strides {st})")
     return t.data_ptr(), dims[-1][1] if dims else size[-1]
+
+
+def _address(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _tokens(dev: int, tokens: torch.Tensor | None, lead: torch.Size) -> tuple[int | None, int]:
+    if tokens is None:
+        return None, 0
+    kind = _TOKEN_TYPES.get(tokens.dtype)
+    if kind is None:
+        raise ValueError(f"tokens: int8, uint8, int32 or int64 required, got {tokens.dtype}")
+    return _like(dev, "tokens", tokens, lead, tokens.dtype), kind
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, n_top: int = 0, ignore_index: int = -100,
@@ -247,24 +276,22 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     (labels of padding) are not read and give 0, alternatives -1.  Returns dict(logprob f32 or None, entropy f32 or None,
     top_ids i32, top_logprob f32 [..., n_top] or None, stats: what `token_logprobs_backward` needs (with `save`; None below STATS_FROM
     classes))."""
-    ptr, stride = _rows(logits, "logits", logits)
-    lead, n_classes = logits.shape[:-1], logits.shape[-1]
-    n = logits.numel() // max(n_classes, 1)
-    dev = logits.device
-    _need(tokens is None or tokens.dtype in _TOKEN_TYPES, "tokens: int8, uint8, int32 or int64 required")
-    tok = None if tokens is None else _like(logits, "tokens", tokens, lead, tokens.dtype)
-    logprob = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev) if want_entropy else None
-    stats = torch.empty((n, 3), dtype=torch.float32, device=dev) if save and n_classes >= STATS_FROM else None
-    ids = torch.empty((*lead, n_top), dtype=torch.int32, device=dev) if n_top > 0 else None
-    top = torch.empty((*lead, n_top), dtype=torch.float32, device=dev) if n_top > 0 else None
+    dev = _device_of("logits", logits)
+    ptr, stride = _rows(dev, "logits", logits)
+    lead, n_classes, dtype, device = logits.shape[:-1], logits.shape[-1], logits.dtype, logits.device
+    n = logits.numel() // n_classes if n_classes else 0
+    tok, kind = _tokens(dev, tokens, lead)
+    logprob = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=device)
+    entropy = torch.empty(lead, dtype=torch.float32, device=device) if want_entropy else None
+    stats = torch.empty((n, 3), dtype=torch.float32, device=device) if save and n_classes >= STATS_FROM else None
+    ids = torch.empty((*lead, n_top), dtype=torch.int32, device=device) if n_top > 0 else None
+    top = torch.empty((*lead, n_top), dtype=torch.float32, device=device) if n_top > 0 else None
     L = _lib.lib()
-    with _on(logits):
-        nb = L.dc_token_logprobs_workspace(n, n_classes, n_top)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        _lib.check(L.dc_token_logprobs(
-            _stream(), ptr, _DTYPES[logits.dtype], n, n_classes, stride, tok, 0 if tokens is None else _TOKEN_TYPES[tokens.dtype], ignore_index,
-            n_top, _ptr(logprob), _ptr(entropy), _ptr(stats), _ptr(ids), _ptr(top), _ptr(ws), nb))
+    nb = L.dc_token_logprobs_workspace(n, n_classes, n_top) if n_classes >= STATS_FROM else 0
+    ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
+    with _on(dev):
+        _lib.check(L.dc_token_logprobs(_stream_of(dev), ptr, _DTYPES[dtype], n, n_classes, stride, tok, kind, ignore_index, n_top, _address(logprob),
+                                       _address(entropy), _address(stats), _address(ids), _address(top), _address(ws), nb))
     return {"logprob": logprob, "entropy": entropy, "top_ids": ids, "top_logprob": top, "stats": stats}
 
 
@@ -272,23 +299,22 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor | None, s
                             grad_entropy: torch.Tensor | None = None, *, ignore_index: int = -100) -> torch.Tensor:
     """Gradient of the logits for gradients of `token_logprobs`' logprob and entropy (either None: zero); `stats` as it
     returned them with `save=True`."""
-    ptr, stride = _rows(logits, "logits", logits)
+    dev = _device_of("logits", logits)
+    ptr, stride = _rows(dev, "logits", logits)
     lead, n_classes = logits.shape[:-1], logits.shape[-1]
-    n = logits.numel() // max(n_classes, 1)
-    _need(tokens is None or tokens.dtype in _TOKEN_TYPES, "tokens: int8, uint8, int32 or int64 required")
-    tok = None if tokens is None else _like(logits, "tokens", tokens, lead, tokens.dtype)
-    st = _like(logits, "stats", stats, (n, 3), torch.float32)
-    gl = _like(logits, "grad_logprob", grad_logprob, lead, torch.float32)
-    gh = _like(logits, "grad_entropy", grad_entropy, lead, torch.float32)
+    n = logits.numel() // n_classes if n_classes else 0
+    tok, kind = _tokens(dev, tokens, lead)
+    st = _like(dev, "stats", stats, (n, 3), torch.float32)
+    gl = _like(dev, "grad_logprob", grad_logprob, lead, torch.float32)
+    gh = _like(dev, "grad_entropy", grad_entropy, lead, torch.float32)
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    with _on(logits):
-        _lib.check(_lib.lib().dc_token_logprobs_backward(
-            _stream(), ptr, _DTYPES[logits.dtype], n, n_classes, stride, tok, 0 if tokens is None else _TOKEN_TYPES[tokens.dtype], ignore_index, st,
-            gl, gh, out.data_ptr(), n_classes))
+    with _on(dev):
+        _lib.check(_lib.lib().dc_token_logprobs_backward(_stream_of(dev), ptr, _DTYPES[logits.dtype], n, n_classes, stride, tok, kind, ignore_index, st,
+                                                         gl, gh, out.data_ptr(), n_classes))
     return out
 
 
-def _scan_shape(x: torch.Tensor, offsets, begin, end, max_len):
+def _scan_shape(dev: int, x: torch.Tensor, offsets, begin, end, max_len):
     """(tokens, channels, sequences, longest, address of begin, of end) of a gated_scan call."""
     if offsets is None and begin is None and end is None:
         _need(x.dim() == 3, "x: [n_seqs, length, n_channels] required without offsets")
@@ -298,11 +324,11 @@ def _scan_shape(x: torch.Tensor, offsets, begin, end, max_len):
     if offsets is not None:
         _need(offsets.dim() == 1 and offsets.numel() >= 1, "offsets: int64[n_seqs + 1] required")
         n = offsets.numel() - 1
-        b = _like(x, "offsets", offsets, (n + 1,), torch.int64)
+        b = _like(dev, "offsets", offsets, (n + 1,), torch.int64)
         e = b + 8
     else:
         n = begin.numel()
-        b, e = _like(x, "begin", begin, (n,), torch.int64), _like(x, "end", end, (n,), torch.int64)
+        b, e = _like(dev, "begin", begin, (n,), torch.int64), _like(dev, "end", end, (n,), torch.int64)
     if max_len is None:  # read back: callers that know the longest sequence pass it (and need to inside a graph capture)
         lens = offsets.diff() if offsets is not None else end - begin
         max_len = max(int(lens.max().item()), 0) if n else 0
@@ -319,25 +345,26 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, *, offsets: torch.Tensor | None
     `begin` / `end` int64[n_seqs] (left-padded rows: first column and end of each).  `h0` f32[n_seqs, n_channels] state to start from; `reverse`: from
     the sequences' ends.  `h_last` may be given (`h0` itself: a state kept in place while bases stream in); `out` keeps what stands in
     tokens of no sequence, which are zero otherwise.  Returns dict(y, h_last, saved: for `gated_scan_backward`, with `save`)."""
-    xp, xs = _rows(x, "x", x)
-    fp, fs = _rows(x, "f", f, x.shape, x.dtype)
-    n, c, seqs, longest, b, e = _scan_shape(x, offsets, begin, end, max_len)
-    dev = x.device
-    h0p = _like(x, "h0", h0, (seqs, c), torch.float32)
+    dev = _device_of("x", x)
+    xp, xs = _rows(dev, "x", x)
+    shape, dtype, device = x.shape, x.dtype, x.device
+    fp, fs = _rows(dev, "f", f, shape, dtype)
+    n, c, seqs, longest, b, e = _scan_shape(dev, x, offsets, begin, end, max_len)
+    h0p = _like(dev, "h0", h0, (seqs, c), torch.float32)
     zero_rest = out is None and offsets is not None  # (dense sequences cover every token)
     if out is None:
-        out = (torch.empty if begin is None else torch.zeros)(x.shape, dtype=x.dtype, device=dev)
-    yp, ys = _rows(x, "out", out, x.shape, x.dtype)
+        out = (torch.empty if begin is None else torch.zeros)(shape, dtype=dtype, device=device)
+    yp, ys = _rows(dev, "out", out, shape, dtype)
     if h_last is None:
-        h_last = torch.empty((seqs, c), dtype=torch.float32, device=dev)
-    hp = _like(x, "h_last", h_last, (seqs, c), torch.float32)
+        h_last = torch.empty((seqs, c), dtype=torch.float32, device=device)
+    hp = _like(dev, "h_last", h_last, (seqs, c), torch.float32)
     L = _lib.lib()
-    saved = torch.empty(L.dc_gated_scan_saved(n, c), dtype=torch.float32, device=dev) if save else None
-    with _on(x):
-        nb = L.dc_gated_scan_workspace(n, c, seqs, longest)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        _lib.check(L.dc_gated_scan(_stream(), _DTYPES[x.dtype], xp, xs, fp, fs, n, c, b, e, seqs, longest, int(reverse), h0p, yp, ys, int(zero_rest),
-                                   hp, _ptr(saved), _ptr(ws), nb))
+    saved = torch.empty(L.dc_gated_scan_saved(n, c), dtype=torch.float32, device=device) if save else None
+    nb = L.dc_gated_scan_workspace(n, c, seqs, longest) if longest > 1 else 0
+    ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
+    with _on(dev):
+        _lib.check(L.dc_gated_scan(_stream_of(dev), _DTYPES[dtype], xp, xs, fp, fs, n, c, b, e, seqs, longest, int(reverse), h0p, yp, ys, int(zero_rest),
+                                   hp, _address(saved), _address(ws), nb))
     return {"y": out, "h_last": h_last, "saved": saved}
 
 
@@ -346,23 +373,24 @@ def gated_scan_backward(x: torch.Tensor, f: torch.Tensor, saved: torch.Tensor, g
                         end: torch.Tensor | None = None, max_len: int | None = None, reverse: bool = False) -> dict:
     """Gradients of `gated_scan` for `grad_y` (and `grad_h_last`): dict(grad_x, grad_f, grad_h0 f32[n_seqs, n_channels]).  The other
     arguments as in the forward call, `saved` as it returned it; tokens of no sequence get zeros."""
-    xp, xs = _rows(x, "x", x)
-    fp, fs = _rows(x, "f", f, x.shape, x.dtype)
-    gp, gs = _rows(x, "grad_y", grad_y, x.shape, x.dtype)
-    n, c, seqs, longest, b, e = _scan_shape(x, offsets, begin, end, max_len)
-    dev = x.device
+    dev = _device_of("x", x)
+    xp, xs = _rows(dev, "x", x)
+    shape, dtype, device = x.shape, x.dtype, x.device
+    fp, fs = _rows(dev, "f", f, shape, dtype)
+    gp, gs = _rows(dev, "grad_y", grad_y, shape, dtype)
+    n, c, seqs, longest, b, e = _scan_shape(dev, x, offsets, begin, end, max_len)
     L = _lib.lib()
-    h0p = _like(x, "h0", h0, (seqs, c), torch.float32)
-    glp = _like(x, "grad_h_last", grad_h_last, (seqs, c), torch.float32)
-    sp = _like(x, "saved", saved, (L.dc_gated_scan_saved(n, c),), torch.float32)
+    h0p = _like(dev, "h0", h0, (seqs, c), torch.float32)
+    glp = _like(dev, "grad_h_last", grad_h_last, (seqs, c), torch.float32)
+    sp = _like(dev, "saved", saved, (L.dc_gated_scan_saved(n, c),), torch.float32)
     make = torch.empty if begin is None else torch.zeros
-    gx, gf = make(x.shape, dtype=x.dtype, device=dev), make(x.shape, dtype=x.dtype, device=dev)
-    gh = torch.empty((seqs, c), dtype=torch.float32, device=dev)
-    with _on(x):
-        nb = L.dc_gated_scan_workspace(n, c, seqs, longest)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-        _lib.check(L.dc_gated_scan_backward(_stream(), _DTYPES[x.dtype], xp, xs, fp, fs, n, c, b, e, seqs, longest, int(reverse), h0p, sp, gp, gs,
-                                            glp, gx.data_ptr(), c, gf.data_ptr(), c, int(offsets is not None), gh.data_ptr(), _ptr(ws), nb))
+    gx, gf = make(shape, dtype=dtype, device=device), make(shape, dtype=dtype, device=device)
+    gh = torch.empty((seqs, c), dtype=torch.float32, device=device)
+    nb = L.dc_gated_scan_workspace(n, c, seqs, longest)
+    ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
+    with _on(dev):
+        _lib.check(L.dc_gated_scan_backward(_stream_of(dev), _DTYPES[dtype], xp, xs, fp, fs, n, c, b, e, seqs, longest, int(reverse), h0p, sp, gp, gs,
+                                            glp, gx.data_ptr(), c, gf.data_ptr(), c, int(offsets is not None), gh.data_ptr(), _address(ws), nb))
     return {"grad_x": gx, "grad_f": gf, "grad_h0": gh}
 
 
@@ -370,6 +398,12 @@ def _norm_ref(y, residual) -> torch.Tensor:
     ref = y if y is not None else residual
     _need(ref is not None, "block_norm: a block's output or a residual is required")
     return ref
+
+
+def _norm_codes(kind: str, gate_act: str) -> tuple[int, int]:
+    if kind not in _NORM_KINDS or gate_act not in _GATE_ACTS:
+        raise ValueError(f"kind is one of {sorted(_NORM_KINDS)}, gate_act one of {sorted(_GATE_ACTS)}; got {kind!r}, {gate_act!r}")
+    return _NORM_KINDS[kind], _GATE_ACTS[gate_act]
 
 
 def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None = None, gate: torch.Tensor | None = None, *, kind: str = "layer",
@@ -383,26 +417,29 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None = None, gat
     "layer" or "rms", gates "identity", "sigmoid" or "silu"; weights, biases and `scale` are float32[width].  `dtype`: of n where y is
     None (default: the residual's); `out`: where r' goes (`residual` itself: in place).  Returns dict(residual: r', normed: n or None)."""
     ref = _norm_ref(y, residual)
-    _need(kind in _NORM_KINDS, f"kind: one of {sorted(_NORM_KINDS)}")
-    _need(gate_act in _GATE_ACTS, f"gate_act: one of {sorted(_GATE_ACTS)}")
+    dev = _device_of("residual" if y is None else "y", ref)
+    k, act = _norm_codes(kind, gate_act)
     act_dtype = y.dtype if y is not None else dtype or ref.dtype
     res_dtype = residual.dtype if residual is not None else act_dtype
-    _need(act_dtype in _DTYPES, f"{act_dtype} is not float32, float16 or bfloat16")
+    _need(act_dtype in _DTYPES, "block_norm: float32, float16 or bfloat16 required")
     _need(gate is None or y is not None, "gate: without a block's output")
-    shape, w = ref.shape, ref.shape[-1]
-    yp, ys = _rows(ref, "y", y, shape)
-    gp, gs = _rows(ref, "gate", gate, shape, act_dtype)
-    rp, rs = _rows(ref, "residual", residual, shape)
-    vec = [_like(ref, n, t, (w,), torch.float32) for n, t in (("scale", scale), ("post_weight", post_weight), ("post_bias", post_bias),
-                                                            ("pre_weight", pre_weight), ("pre_bias", pre_bias))]
+    shape, device = ref.shape, ref.device
+    w = shape[-1]
+    yp, ys = _rows(dev, "y", y, shape)
+    gp, gs = _rows(dev, "gate", gate, shape, act_dtype)
+    rp, rs = _rows(dev, "residual", residual, shape)
+    one = (w,)
+    sc = _like(dev, "scale", scale, one, torch.float32)
+    pw, pb = _like(dev, "post_weight", post_weight, one, torch.float32), _like(dev, "post_bias", post_bias, one, torch.float32)
+    qw, qb = _like(dev, "pre_weight", pre_weight, one, torch.float32), _like(dev, "pre_bias", pre_bias, one, torch.float32)
     if out is None and y is not None:
-        out = torch.empty(shape, dtype=res_dtype, device=ref.device)
-    op, os_ = _rows(ref, "out", out, shape, res_dtype)
-    normed = torch.empty(shape, dtype=act_dtype, device=ref.device) if pre else None
-    with _on(ref):
+        out = torch.empty(shape, dtype=res_dtype, device=device)
+    op, os_ = _rows(dev, "out", out, shape, res_dtype)
+    normed = torch.empty(shape, dtype=act_dtype, device=device) if pre else None
+    with _on(dev):
         _lib.check(_lib.lib().dc_block_norm(
-            _stream(), _DTYPES[act_dtype], _DTYPES.get(res_dtype, -1), ref.numel() // max(w, 1), w, _NORM_KINDS[kind], eps, yp, ys, gp, gs,
-            _GATE_ACTS[gate_act], rp, rs, vec[0], int(post), vec[1], vec[2], vec[3], vec[4], op, os_, _ptr(normed), w))
+            _stream_of(dev), _DTYPES[act_dtype], _DTYPES[res_dtype], ref.numel() // w if w else 0, w, k, eps, yp, ys, gp, gs, act, rp, rs, sc,
+            int(post), pw, pb, qw, qb, op, os_, _address(normed), w))
     return {"residual": residual if out is None else out, "normed": normed}
 
 
@@ -415,39 +452,41 @@ def block_norm_backward(y: torch.Tensor | None, residual: torch.Tensor | None = 
     arguments as in the forward call, `residual` as it was BEFORE it.  Returns dict(grad_y, grad_gate, grad_residual, and float32[width]
     grad_scale, grad_post_weight, grad_post_bias, grad_pre_weight, grad_pre_bias); None for what the call did not have."""
     ref = _norm_ref(y, residual)
-    _need(kind in _NORM_KINDS, f"kind: one of {sorted(_NORM_KINDS)}")
-    _need(gate_act in _GATE_ACTS, f"gate_act: one of {sorted(_GATE_ACTS)}")
+    dev = _device_of("residual" if y is None else "y", ref)
+    k, act = _norm_codes(kind, gate_act)
     act_dtype = y.dtype if y is not None else grad_normed.dtype if grad_normed is not None else ref.dtype
     res_dtype = residual.dtype if residual is not None else act_dtype
-    _need(act_dtype in _DTYPES, f"{act_dtype} is not float32, float16 or bfloat16")
+    _need(act_dtype in _DTYPES, "block_norm: float32, float16 or bfloat16 required")
     _need(gate is None or y is not None, "gate: without a block's output")
-    shape, w, dev = ref.shape, ref.shape[-1], ref.device
-    n = ref.numel() // max(w, 1)
-    yp, ys = _rows(ref, "y", y, shape)
-    gp, gs = _rows(ref, "gate", gate, shape, act_dtype)
-    rp, rs = _rows(ref, "residual", residual, shape)
-    grp, grs = _rows(ref, "grad_residual", grad_residual, shape, res_dtype)
-    gnp, gns = _rows(ref, "grad_normed", grad_normed, shape, act_dtype)
-    vec = [_like(ref, m, t, (w,), torch.float32) for m, t in (("scale", scale), ("post_weight", post_weight), ("post_bias", post_bias),
-                                                            ("pre_weight", pre_weight))]
-    _like(ref, "pre_bias", pre_bias, (w,), torch.float32)
+    shape, device = ref.shape, ref.device
+    w = shape[-1]
+    n = ref.numel() // w if w else 0
+    yp, ys = _rows(dev, "y", y, shape)
+    gp, gs = _rows(dev, "gate", gate, shape, act_dtype)
+    rp, rs = _rows(dev, "residual", residual, shape)
+    grp, grs = _rows(dev, "grad_residual", grad_residual, shape, res_dtype)
+    gnp, gns = _rows(dev, "grad_normed", grad_normed, shape, act_dtype)
+    one = (w,)
+    sc = _like(dev, "scale", scale, one, torch.float32)
+    pw, pb = _like(dev, "post_weight", post_weight, one, torch.float32), _like(dev, "post_bias", post_bias, one, torch.float32)
+    qw = _like(dev, "pre_weight", pre_weight, one, torch.float32)
+    _like(dev, "pre_bias", pre_bias, one, torch.float32)
 
     def grad(like, dt=torch.float32):
-        return None if like is None else torch.empty(like.shape, dtype=dt, device=dev)
+        return None if like is None else torch.empty(like.shape, dtype=dt, device=device)
 
     normed = post and y is not None
     g = {"grad_y": grad(y, act_dtype), "grad_gate": grad(gate, act_dtype), "grad_residual": grad(residual, res_dtype),
          "grad_scale": grad(scale) if y is not None else None, "grad_post_weight": grad(post_weight) if normed else None,
          "grad_post_bias": grad(post_bias) if normed else None, "grad_pre_weight": grad(pre_weight), "grad_pre_bias": grad(pre_bias)}
     L = _lib.lib()
-    with _on(ref):
-        nb = L.dc_block_norm_workspace(n, w)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    nb = L.dc_block_norm_workspace(n, w)
+    ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
+    with _on(dev):
         _lib.check(L.dc_block_norm_backward(
-            _stream(), _DTYPES[act_dtype], _DTYPES.get(res_dtype, -1), n, w, _NORM_KINDS[kind], eps, yp, ys, gp, gs, _GATE_ACTS[gate_act], rp, rs,
-            vec[0], int(post), vec[1], vec[2], vec[3], grp, grs, gnp, gns, _ptr(g["grad_y"]), _ptr(g["grad_gate"]), _ptr(g["grad_residual"]),
-            _ptr(g["grad_scale"]), _ptr(g["grad_post_weight"]), _ptr(g["grad_post_bias"]), _ptr(g["grad_pre_weight"]), _ptr(g["grad_pre_bias"]),
-            _ptr(ws), nb))
+            _stream_of(dev), _DTYPES[act_dtype], _DTYPES[res_dtype], n, w, k, eps, yp, ys, gp, gs, act, rp, rs, sc, int(post), pw, pb, qw, grp, grs,
+            gnp, gns, *(_address(g[m]) for m in ("grad_y", "grad_gate", "grad_residual", "grad_scale", "grad_post_weight", "grad_post_bias",
+                                                 "grad_pre_weight", "grad_pre_bias")), _address(ws), nb))
     return g
 
 
