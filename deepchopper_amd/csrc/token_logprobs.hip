@@ -92,6 +92,12 @@ __device__ __forceinline__ void load_few(const T* row, int n, int lane, int bits
   }
 }
 
+// log(1 + s) for s >= 0 to the last digits of s: what 1 + s rounds away comes back as c / (1 + s)
+__device__ __forceinline__ float log_one_plus(float s) {
+  const float u = 1.0f + s, c = s - (u - 1.0f);
+  return __builtin_fmaf(c, fast_rcp(u), __builtin_amdgcn_logf(u) * kLn2);
+}
+
 template <int E>
 __device__ __forceinline__ RowStats few_stats(const Few<E>& f, int bits) {
   float m = f.z[0];
@@ -112,15 +118,16 @@ __device__ __forceinline__ RowStats few_stats(const Few<E>& f, int bits) {
   u = lanes_sum(u, bits);
   if (m == -INFINITY && s == 0.0f) return {m, 0.0f, 0.0f};
   s += ones - 1.0f;
-  const float log_sum = log1pf(s);
+  const float log_sum = log_one_plus(s);
   return {ref, log_sum, log_sum - u * fast_rcp(1.0f + s)};
 }
 
-template <typename T, int E>
-__global__ __launch_bounds__(256) void few_classes_kernel(const T* __restrict__ logits, int64_t n_rows, int32_t n, int64_t ld, int32_t bits, Tokens tok,
+// ONE: a row is one lane's (bits = 0, known to the compiler)
+template <typename T, int E, bool ONE>
+__global__ __launch_bounds__(256) void few_classes_kernel(const T* __restrict__ logits, int64_t n_rows, int32_t n, int64_t ld, int32_t lane_bits, Tokens tok,
                                                           int32_t n_top, float* __restrict__ logprob, float* __restrict__ entropy,
                                                           float* __restrict__ stats, int32_t* __restrict__ top_ids, float* __restrict__ top_logprob) {
-  const int lane = threadIdx.x & ((1 << bits) - 1);
+  const int bits = ONE ? 0 : lane_bits, lane = threadIdx.x & ((1 << bits) - 1);
   const int64_t step = (int64_t)gridDim.x * (256 >> bits);
   for (int64_t i = (int64_t)blockIdx.x * (256 >> bits) + (threadIdx.x >> bits); i < n_rows; i += step) {
     const int64_t t = tok.p ? token_at(tok, i) : 0;
@@ -174,12 +181,12 @@ __global__ __launch_bounds__(256) void few_classes_kernel(const T* __restrict__ 
   }
 }
 
-template <typename T, int E>
-__global__ __launch_bounds__(256) void few_classes_backward_kernel(const T* logits, int64_t n_rows, int32_t n, int64_t ld, int32_t bits, Tokens tok,
+template <typename T, int E, bool ONE>
+__global__ __launch_bounds__(256) void few_classes_backward_kernel(const T* logits, int64_t n_rows, int32_t n, int64_t ld, int32_t lane_bits, Tokens tok,
                                                                    const float* __restrict__ g_logprob, const float* __restrict__ g_entropy, T* out,
                                                                    int64_t ld_out) {
   constexpr int W = Few<E>::W;
-  const int lane = threadIdx.x & ((1 << bits) - 1);
+  const int bits = ONE ? 0 : lane_bits, lane = threadIdx.x & ((1 << bits) - 1);
   const int64_t step = (int64_t)gridDim.x * (256 >> bits);
   for (int64_t i = (int64_t)blockIdx.x * (256 >> bits) + (threadIdx.x >> bits); i < n_rows; i += step) {
     const int64_t t = tok.p ? token_at(tok, i) : -1;
@@ -231,26 +238,26 @@ struct Layout {
   }
 };
 
-// max, S and U about it (U in powers of two); m = -inf, S = 0: nothing yet
+// The maximum m, and S = sum 2^d, U = sum 2^d d over d = (z - m) log2(e); m = -inf, S = 0: nothing yet.  (The difference is taken first:
+// z log2(e) - m log2(e) in one FMA would overflow for logits of the type's lowest value.)
 struct Running {
   float m, s, u;
 };
-__device__ __forceinline__ Running merged(const Running& a, const Running& b) {
-  const float m = __builtin_fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.0f : m;
-  Running r{m, 0.0f, 0.0f};
-  for (const Running& x : {a, b}) {
-    // (S of a part that has seen only -inf is 0, or NaN; below 2^-200 a part counts for nothing, and 0 x -inf is not wanted)
-    const float d = x.m == -INFINITY ? 0.0f : __builtin_fmaxf((x.m - ref) * kLog2e, -200.0f);
-    const float f = fast_exp2(d);
-    r.s = __builtin_fmaf(f, x.s, r.s);
-    r.u = __builtin_fmaf(f, __builtin_fmaf(d, x.s, x.u), r.u);
-  }
-  return r;
+// x's sums moved to the maximum m >= x.m.  (S of a part that has seen only -inf is 0, or NaN; 2^-200 counts for nothing, and 0 x -inf is
+// not wanted.)
+__device__ __forceinline__ Running moved(const Running& x, float m) {
+  const float ref = m == -INFINITY ? 0.0f : m;
+  const float d = x.m == -INFINITY ? 0.0f : __builtin_fmaxf((x.m - ref) * kLog2e, -200.0f), f = fast_exp2(d);
+  return {m, f * x.s, f * __builtin_fmaf(d, x.s, x.u)};
 }
-__device__ __forceinline__ Running wave_merged(Running r) {
-  const float m = lanes_max(r.m, 6), ref = m == -INFINITY ? 0.0f : m;
-  const float d = r.m == -INFINITY ? 0.0f : __builtin_fmaxf((r.m - ref) * kLog2e, -200.0f), f = fast_exp2(d);
-  return {m, wave_sum(f * r.s), wave_sum(f * __builtin_fmaf(d, r.s, r.u))};
+__device__ __forceinline__ Running merged(const Running& a, const Running& b) {
+  const float m = __builtin_fmaxf(a.m, b.m);
+  const Running x = moved(a, m), y = moved(b, m);
+  return {m, x.s + y.s, x.u + y.u};
+}
+__device__ __forceinline__ Running wave_merged(const Running& r) {
+  const Running x = moved(r, lanes_max(r.m, 6));
+  return {x.m, wave_sum(x.s), wave_sum(x.u)};
 }
 __device__ __forceinline__ RowStats finish(const Running& r) {
   if (r.m == -INFINITY && r.s == 0.0f) return {r.m, 0.0f, 0.0f};
@@ -264,8 +271,9 @@ struct Candidates {
   int n, k;        // collected, wanted
   float bound;     // a class below it is none of the k best
   uint64_t worst;  // the k-th best of those ranked so far, or 0
+  int ranked;      // how many at the list's front are in order already
 
-  __device__ __forceinline__ void start(uint64_t* lds, int wanted) { list = lds, n = 0, k = wanted, bound = -INFINITY, worst = 0; }
+  __device__ __forceinline__ void start(uint64_t* lds, int wanted) { list = lds, n = 0, k = wanted, bound = -INFINITY, worst = 0, ranked = 0; }
 
   // the lanes of `has` add theirs; a full list is ranked first
   __device__ __forceinline__ void add(bool has, uint64_t cand) {
@@ -282,13 +290,20 @@ struct Candidates {
 
   // the k best, in order, to the front of the list: everyone counts how many are better than its one or two
   __device__ void rank() {
+    if (n == ranked) return;
     const int lane = threadIdx.x & 63;
     __builtin_amdgcn_wave_barrier();
     const uint64_t a = lane < n ? list[lane] : 0, b = lane + 64 < n ? list[lane + 64] : 0;
     int ra = 0, rb = 0;
-    for (int i = 0; i < n; ++i) {
-      const uint64_t o = list[i];
-      ra += o > a, rb += o > b;
+    if (n <= 64) {
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) ra += list[i] > a;
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const uint64_t o = list[i];
+        ra += o > a, rb += o > b;
+      }
     }
     __builtin_amdgcn_wave_barrier();
     if (lane < n && ra < k) list[ra] = a;
@@ -300,6 +315,7 @@ struct Candidates {
       const float v = key_value((uint32_t)(worst >> 32));
       bound = v;  // (a NaN bound lets every class through to the comparison with `worst`)
     }
+    ranked = n;
   }
 };
 __device__ __forceinline__ uint64_t candidate(float z, int c) { return (uint64_t)order_key(z) << 32 | (uint32_t)~c; }
@@ -392,7 +408,7 @@ __global__ __launch_bounds__(256) void many_classes_kernel(const T* __restrict__
     auto fetch = [&](int v) {
 #pragma unroll
       for (int q = 0; q < kVectors; ++q)
-        if (v + q * 64 + lane < v1) raw[q] = vecs[v + q * 64 + lane];
+        raw[q] = v + q * 64 + lane < v1 ? vecs[v + q * 64 + lane] : Vec((T)-INFINITY);
     };
     fetch(v0);
     Running r{-INFINITY, 0.0f, 0.0f};
@@ -410,9 +426,8 @@ __global__ __launch_bounds__(256) void many_classes_kernel(const T* __restrict__
       float z[kVectors][W];
 #pragma unroll
       for (int q = 0; q < kVectors; ++q) {
-        const bool in = v + q * 64 + lane < v1;
 #pragma unroll
-        for (int w = 0; w < W; ++w) z[q][w] = in ? (float)raw[q][w] : -INFINITY;
+        for (int w = 0; w < W; ++w) z[q][w] = (float)raw[q][w];
       }
       if (v + 64 * kVectors < v1) fetch(v + 64 * kVectors);
       float pm = z[0][0];
@@ -421,10 +436,7 @@ __global__ __launch_bounds__(256) void many_classes_kernel(const T* __restrict__
 #pragma unroll
         for (int w = 0; w < W; ++w) pm = __builtin_fmaxf(pm, z[q][w]);
       if (!(pm <= r.m)) {  // the lane's maximum moves
-        const float ref = pm == -INFINITY ? 0.0f : pm, d = r.m == -INFINITY ? 0.0f : __builtin_fmaxf((r.m - ref) * kLog2e, -200.0f), f = fast_exp2(d);
-        r.u = f * __builtin_fmaf(d, r.s, r.u);
-        r.s *= f;
-        r.m = __builtin_fmaxf(pm, r.m);
+        r = moved(r, __builtin_fmaxf(pm, r.m));
       }
       const float ref = r.m == -INFINITY ? 0.0f : r.m;
 #pragma unroll
@@ -433,7 +445,7 @@ __global__ __launch_bounds__(256) void many_classes_kernel(const T* __restrict__
         for (int w = 0; w < W; ++w) {
           const float d = (z[q][w] - ref) * kLog2e, e = fast_exp2(d);
           r.s += e;
-          r.u = __builtin_fmaf(e, __builtin_fmaxf(d, -200.0f), r.u);  // (e is 0 there, and 0 x -inf is not wanted)
+          r.u = __builtin_fmaf(e, __builtin_fmaxf(d, -200.0f), r.u);
         }
       }
       if constexpr (TOP) {
@@ -446,8 +458,8 @@ __global__ __launch_bounds__(256) void many_classes_kernel(const T* __restrict__
           const bool in = v + q * 64 + lane < v1;
 #pragma unroll
           for (int w = 0; w < W; ++w) {
-            const bool may = in && !(z[q][w] < best.bound);
-            if (__ballot(may)) best.add(may, candidate(z[q][w], at.head + (v + q * 64 + lane) * W + w));
+            const bool may = !(z[q][w] < best.bound);
+            if (__ballot(may)) best.add(may && in, candidate(z[q][w], at.head + (v + q * 64 + lane) * W + w));
           }
         }
         if (v == v0) best.rank();
@@ -495,13 +507,15 @@ __global__ __launch_bounds__(64) void join_slices_kernel(const T* __restrict__ l
     Candidates best;
     if (n_top > 0) {
       best.start(lds, n_top);
-      const uint64_t* from = sl.best + i * sl.n * n_top;
-      const uint64_t top = lane < sl.n ? from[lane * n_top] : 0;  // (0: no candidate)
-      const float b = first_bound(top ? key_value((uint32_t)(top >> 32)) : -INFINITY, n_top);
-      for (int c = 0; c < sl.n * n_top; c += 64) {
-        const uint64_t cand = c + lane < sl.n * n_top ? from[c + lane] : 0;
-        const bool may = cand != 0 && !(key_value((uint32_t)(cand >> 32)) < b);
-        if (__ballot(may)) best.add(may, cand);
+      // a lane holds a slice: its candidates come in order, so it is done at the first one below the bound
+      const uint64_t* from = sl.best + (i * sl.n + (lane < sl.n ? lane : 0)) * n_top;
+      uint64_t cand = lane < sl.n ? from[0] : 0;  // (0: no candidate)
+      best.bound = first_bound(cand ? key_value((uint32_t)(cand >> 32)) : -INFINITY, n_top);
+      for (int q = 0; q < n_top; ++q) {
+        const bool may = cand != 0 && !(key_value((uint32_t)(cand >> 32)) < best.bound);
+        if (!__ballot(may)) break;
+        best.add(may, cand);
+        cand = may && q + 1 < n_top ? from[q + 1] : 0;
       }
       best.rank();
     }
@@ -585,8 +599,9 @@ int lane_bits_of(int32_t n_classes) {
 template <typename F>
 int with_few(int32_t dtype, int32_t n_classes, F&& f) {
   return with_dtype(dtype, [&](auto t) {
-    if (n_classes <= 2) return f(t, std::integral_constant<int, 2>{});
-    return n_classes <= 256 ? f(t, std::integral_constant<int, 4>{}) : f(t, std::integral_constant<int, 8>{});
+    if (n_classes <= 2) return f(t, std::integral_constant<int, 2>{}, std::true_type{});
+    if (n_classes <= 4) return f(t, std::integral_constant<int, 4>{}, std::true_type{});
+    return n_classes <= 256 ? f(t, std::integral_constant<int, 4>{}, std::false_type{}) : f(t, std::integral_constant<int, 8>{}, std::false_type{});
   });
 }
 
@@ -624,9 +639,9 @@ extern "C" int dc_token_logprobs(void* stream, const void* d_logits, int32_t dty
   const Tokens tok{d_tokens, token_type, ignore_token};
   if (n_classes < DC_STATS_FROM) {
     const int bits = lane_bits_of(n_classes);
-    return with_few(dtype, n_classes, [&](auto t, auto e) {
+    return with_few(dtype, n_classes, [&](auto t, auto e, auto one) {
       using T = decltype(t);
-      few_classes_kernel<T, decltype(e)::value><<<dim3(grid_of((n_rows + (256 >> bits) - 1) / (256 >> bits))), dim3(256), 0, as_stream(stream)>>>(
+      few_classes_kernel<T, decltype(e)::value, decltype(one)::value><<<dim3(grid_of((n_rows + (256 >> bits) - 1) / (256 >> bits))), dim3(256), 0, as_stream(stream)>>>(
           (const T*)d_logits, n_rows, n_classes, row_stride, bits, tok, n_top, d_logprob, d_entropy, d_stats, d_top_ids, d_top_logprob);
       DC_LAUNCH_CHECK();
       return DC_OK;
@@ -664,9 +679,9 @@ extern "C" int dc_token_logprobs_backward(void* stream, const void* d_logits, in
   const Tokens tok{d_tokens, token_type, ignore_token};
   if (n_classes < DC_STATS_FROM) {
     const int bits = lane_bits_of(n_classes);
-    return with_few(dtype, n_classes, [&](auto t, auto e) {
+    return with_few(dtype, n_classes, [&](auto t, auto e, auto one) {
       using T = decltype(t);
-      few_classes_backward_kernel<T, decltype(e)::value><<<dim3(grid_of((n_rows + (256 >> bits) - 1) / (256 >> bits))), dim3(256), 0, as_stream(stream)>>>(
+      few_classes_backward_kernel<T, decltype(e)::value, decltype(one)::value><<<dim3(grid_of((n_rows + (256 >> bits) - 1) / (256 >> bits))), dim3(256), 0, as_stream(stream)>>>(
           (const T*)d_logits, n_rows, n_classes, row_stride, bits, tok, d_grad_logprob, d_grad_entropy, (T*)d_grad_logits, grad_stride);
       DC_LAUNCH_CHECK();
       return DC_OK;
