@@ -61,12 +61,9 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }    // v_rcp_f32: 1 ulp
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-// p = min(sigmoid(f), 1 - sigmoid(f)) = e / (1 + e) with e = exp(-|f|): of the two weights of a gate the one that has full
-// relative accuracy; the other is 1 - p.
-__device__ __forceinline__ float gate_minor(float f) {
-  const float e = fast_exp2(-__builtin_fabsf(f) * kLog2e);
-  return e * fast_rcp(1.0f + e);
-}
+// p = min(sigmoid(f), 1 - sigmoid(f)) = 1 / (1 + exp(|f|)): of the two weights of a gate the one that has full relative accuracy; the
+// other is 1 - p.
+__device__ __forceinline__ float gate_minor(float f) { return fast_rcp(1.0f + fast_exp2(__builtin_fabsf(f) * kLog2e)); }
 
 // The value of another lane by a fixed pattern of lanes, without a trip through LDS.
 template <int CTRL>

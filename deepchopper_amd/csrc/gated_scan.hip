@@ -1,7 +1,7 @@
 // dc_gated_scan: h_t = a_t h_(t-1) + (1 - a_t) x_t with a = sigmoid(f), per channel of every sequence, and its backward pass.
 //
 // Arithmetic.  A gate has two weights, a and 1 - a, and fp32 holds only the smaller of them to full relative accuracy:
-// p = min(a, 1 - a) = e / (1 + e), e = exp(-|f|).  Each step is a move by p from one operand towards the other,
+// p = min(a, 1 - a) = 1 / (1 + exp(|f|)).  Each step is a move by p from one operand towards the other,
 //   f > 0: h' = h + p (x - h)        f <= 0: h' = x - p (x - h)
 // so a gate that keeps 99.99 % for thousands of tokens loses no more than one that forgets at once (with a rounded, a h would
 // drift by 2^-25 a step).  A span of steps is the map h -> H + A h; it carries both A and G = 1 - A and is applied with the
@@ -35,7 +35,14 @@ struct ScanArgs {
   int32_t n_chunks;   // chunks of a sequence ...
   int64_t chunk;      // ... of so many tokens each (a multiple of the workgroup's tile)
   int32_t n_blocks;   // workgroups of the recurrence; those behind them write the zeros of zero_rest
+  int32_t whole;      // every lane has channels and all strides are at most 2^20: tiles inside a sequence need no checks
 };
+
+// a value that is the same in all lanes, into scalar registers
+__device__ __forceinline__ int64_t scalar(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
 
 // A sequence in the order of the recurrence: its token j is row base + dir * j.
 struct Seq {
@@ -43,7 +50,7 @@ struct Seq {
   int32_t dir;
   bool ok;
   __device__ __forceinline__ Seq(const ScanArgs& a, int s) {
-    const int64_t b = a.begin ? a.begin[s] : s * a.max_len, e = a.end ? a.end[s] : b + a.max_len;
+    const int64_t b = scalar(a.begin ? a.begin[s] : s * a.max_len), e = scalar(a.end ? a.end[s] : b + a.max_len);
     ok = b >= 0 && e >= b && e <= a.n_tokens && e - b <= a.max_len;
     len = ok ? e - b : 0;
     base = a.reverse ? e - 1 : b;
@@ -59,6 +66,15 @@ __device__ __forceinline__ float step(float h, float x, float ps) { return __bui
 // a * v
 __device__ __forceinline__ float decay(float v, float ps) { return keeps(ps) ? __builtin_fmaf(-ps, v, v) : -ps * v; }
 
+// Comparisons made of ps so far are not kept (in scalar registers that spill) but made again.
+template <int V>
+__device__ __forceinline__ void forget(float (&ps)[kSteps][V]) {
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+    for (int v = 0; v < V; ++v) asm volatile("" : "+v"(ps[i][v]));
+}
+
 // x where it counts: a gate of +inf (or one whose other weight is 0 in fp32) does not look at it
 __device__ __forceinline__ float seen(float x, float ps) { return __float_as_int(ps) == 0 ? 0.0f : x; }
 
@@ -70,11 +86,10 @@ __device__ __forceinline__ Span identity_span() { return {1.0f, 0.0f, 0.0f}; }
 __device__ __forceinline__ float apply(float A, float G, float H, float h) {
   return A > 0.5f ? h + __builtin_fmaf(-G, h, H) : __builtin_fmaf(A, h, H);
 }
-__device__ __forceinline__ void extend(float& A, float& G, float ps) {  // by one step
-  const float p = __builtin_fabsf(ps), q = 1.0f - p;
-  const bool k = keeps(ps);
-  A *= k ? q : p;
-  G = __builtin_fmaf(k ? p : q, 1.0f - G, G);
+__device__ __forceinline__ void extend(float& A, float& G, float ps) {  // by one step; G is what an input of 1 makes of a state of 0
+  const float t = __builtin_fabsf(ps) * A;
+  A = keeps(ps) ? A - t : t;
+  G = step(G, 1.0f, ps);
 }
 __device__ __forceinline__ Span then(const Span& a, const Span& b) {  // a, then b
   return {a.A * b.A, __builtin_fmaf(b.G, 1.0f - a.G, a.G), apply(b.A, b.G, b.H, a.H)};
@@ -172,10 +187,10 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_backward_kernel(ScanAr
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float ps = signed_gate(fv[v]), p = __builtin_fabsf(ps);
-      const float total = g[v] + yv[v];
-      g[v] = decay(total, ps);
-      ox[v] = keeps(ps) ? p * total : __builtin_fmaf(ps, total, total);
-      of[v] = p * (1.0f - p) * total * above[j][threadIdx.x * V + v];
+      const float total = g[v] + yv[v], part = p * total, rest = __builtin_fmaf(-p, total, total);
+      ox[v] = keeps(ps) ? part : rest;
+      g[v] = keeps(ps) ? rest : part;
+      of[v] = p * rest * above[j][threadIdx.x * V + v];
     }
     store_vec<V>(gx + t * ldgx + c, ox);
     store_vec<V>(gf + t * ldgf + c, of);
@@ -220,6 +235,31 @@ struct Rows {
         r[i] = vec_t<T, V>(0);
       }
     }
+  }
+};
+
+// The rows of a whole tile: a scalar base a row of a group and one 32-bit byte offset a lane (strides up to 2^20: ScanArgs.whole).
+template <typename T, int V>
+struct TileRows {
+  int64_t first, per_step;  // elements from the row of a tile's first token to the lowest row of a group's step 0; from step to step
+  uint32_t lane;            // bytes
+  __device__ __forceinline__ TileRows(const Place<V>& at, const Seq& q, int64_t ld) {
+    const int group = q.dir < 0 ? at.n_groups - 1 - at.group : at.group;
+    first = q.dir < 0 ? -(int64_t)(at.n_groups - 1) * kSteps * ld : 0;
+    per_step = q.dir * ld;
+    lane = ((uint32_t)(group * kSteps) * (uint32_t)ld + (uint32_t)at.channel) * (uint32_t)sizeof(T);
+  }
+  // `tile`: the row of the tile's first token
+  __device__ __forceinline__ void load(const T* tile, Rows<T, V>& to) const {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const char* p = reinterpret_cast<const char*>(tile + first + i * per_step) + lane;
+      if constexpr (V == 1) to.r[i][0] = *reinterpret_cast<const T*>(p);
+      else to.r[i] = *reinterpret_cast<const vec_t<T, V>*>(p);
+    }
+  }
+  __device__ __forceinline__ void store(T* tile, int i, const float (&v)[V]) const {
+    store_vec<V>(reinterpret_cast<T*>(reinterpret_cast<char*>(tile + first + i * per_step) + lane), v);
   }
 };
 
@@ -331,10 +371,10 @@ __device__ void compose_chunks(const ScanArgs& a, const Place<V>& at, const floa
 }
 
 template <typename T, int V>
-__global__ __launch_bounds__(kThreads, 2) void scan_tile_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f, int64_t ldf,
+__global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f, int64_t ldf,
                                                                 const float* h0, T* __restrict__ y, int64_t ldy, float* h_last,
                                                                 float* __restrict__ saved, const float* __restrict__ maps) {
-  __shared__ float lds[2][3][kThreads * V];
+  __shared__ float lds[2][3][kThreads * V], ends[2][64 * V];
   if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, y, ldy, nullptr, 0);
   const Place<V> at(a);
   const Seq q(a, at.s);
@@ -349,14 +389,23 @@ __global__ __launch_bounds__(kThreads, 2) void scan_tile_kernel(ScanArgs a, cons
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = h0 && at.active ? h0[sc + v] : 0.0f;
   }
+  const TileRows<T, V> tx(at, q, ldx), tf(at, q, ldf), ty(at, q, ldy);
   const int64_t sx = q.dir * ldx, sf = q.dir * ldf, sy = q.dir * ldy;
+  const bool last_group = at.group == at.n_groups - 1;
   int turn = 0;
-  for (int64_t jt = j0; jt < j1; jt += tile, turn ^= 1) {
+  auto one_tile = [&](auto whole, int64_t jt) {
+    constexpr bool WHOLE = decltype(whole)::value;
     const int64_t j = jt + at.group * kSteps, left = j1 - j;
-    const int n = !at.active || left <= 0 ? 0 : left < kSteps ? (int)left : kSteps;
+    const int n = WHOLE ? kSteps : !at.active || left <= 0 ? 0 : left < kSteps ? (int)left : kSteps;
     Rows<T, V> rx, rf;
-    rx.load(x + q.row(j) * ldx + at.channel, sx, n);
-    rf.load(f + q.row(j) * ldf + at.channel, sf, n);
+    if constexpr (WHOLE) {
+      const int64_t row = q.row(jt);
+      tx.load(x + row * ldx, rx);
+      tf.load(f + row * ldf, rf);
+    } else {
+      rx.load(x + q.row(j) * ldx + at.channel, sx, n);
+      rf.load(f + q.row(j) * ldf + at.channel, sf, n);
+    }
     float xs[kSteps][V], ps[kSteps][V];
     Span m[V];
 #pragma unroll
@@ -365,7 +414,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_tile_kernel(ScanArgs a, cons
     for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        ps[i][v] = i < n ? signed_gate((float)rf.r[i][v]) : 0.0f;
+        ps[i][v] = WHOLE || i < n ? signed_gate((float)rf.r[i][v]) : 0.0f;
         xs[i][v] = seen((float)rx.r[i][v], ps[i][v]);
         extend(m[v].A, m[v].G, ps[i][v]);
         m[v].H = step(m[v].H, xs[i][v], ps[i][v]);
@@ -376,17 +425,19 @@ __global__ __launch_bounds__(kThreads, 2) void scan_tile_kernel(ScanArgs a, cons
       const int i = at.at(at.group, lanes_v) + v;
       lds[turn][0][i] = m[v].A, lds[turn][1][i] = m[v].G, lds[turn][2][i] = m[v].H;
     }
-    __syncthreads();  // (one a tile: the next tile writes the other half)
+    __syncthreads();  // (one a tile: the next tile writes the other halves)
     float h[V];
-    for (int k = 0; k < at.n_groups; ++k) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = jt == j0 ? carry[v] : ends[turn ^ 1][at.slot + v];
+    for (int k = 0; k < at.group; ++k) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int i = at.at(k, lanes_v) + v;
-        if (k == at.group) h[v] = carry[v];
-        carry[v] = apply(lds[turn][0][i], lds[turn][1][i], lds[turn][2][i], carry[v]);
+        h[v] = apply(lds[turn][0][i], lds[turn][1][i], lds[turn][2][i], h[v]);
       }
     }
-    if (n > 0) {
+    if (WHOLE || n > 0) {
+      forget<V>(ps);
       if (saved && j % kTile == 0 && j > 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) saved[q.row(j) / kTile * a.n_channels + at.channel + v] = h[v];
@@ -396,11 +447,21 @@ __global__ __launch_bounds__(kThreads, 2) void scan_tile_kernel(ScanArgs a, cons
       for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = step(h[v], xs[i][v], ps[i][v]);
-        if (i < n) store_vec<V>(out + i * sy, h);
+        if constexpr (WHOLE) ty.store(y + q.row(jt) * ldy, i, h);
+        else if (i < n) store_vec<V>(out + i * sy, h);
       }
     }
-  }
-  if (h_last && at.group == 0 && at.active && j1 == q.len) {
+    if (last_group) {  // the state behind the tile, for the next one
+#pragma unroll
+      for (int v = 0; v < V; ++v) ends[turn][at.slot + v] = carry[v] = h[v];
+    }
+    turn ^= 1;
+  };
+  int64_t jt = j0;
+  if (a.whole)
+    for (; jt + tile <= j1; jt += tile) one_tile(std::true_type{}, jt);
+  for (; jt < j1; jt += tile) one_tile(std::false_type{}, jt);
+  if (h_last && last_group && at.active && j1 == q.len) {
 #pragma unroll
     for (int v = 0; v < V; ++v) h_last[sc + v] = q.ok ? carry[v] : __builtin_nanf("");
   }
@@ -409,12 +470,12 @@ __global__ __launch_bounds__(kThreads, 2) void scan_tile_kernel(ScanArgs a, cons
 // Tiles from the last one back.  The state a tile was entered with comes from `saved`; maps of the states and of what comes back go
 // through the same exchange.
 template <typename T, int V>
-__global__ __launch_bounds__(kThreads, 2) void scan_tile_backward_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f,
+__global__ __launch_bounds__(kThreads, 4) void scan_tile_backward_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f,
                                                                          int64_t ldf, const float* __restrict__ h0, const float* __restrict__ saved,
                                                                          const T* __restrict__ gy, int64_t ldgy, const float* g_last,
                                                                          T* __restrict__ gx, int64_t ldgx, T* __restrict__ gf, int64_t ldgf, float* g_h0,
                                                                          const float* __restrict__ maps) {
-  __shared__ float lds[2][4][kThreads * V];
+  __shared__ float lds[2][4][kThreads * V], ends[2][64 * V];
   if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, gx, ldgx, gf, ldgf);
   const Place<V> at(a);
   const Seq q(a, at.s);
@@ -431,15 +492,24 @@ __global__ __launch_bounds__(kThreads, 2) void scan_tile_backward_kernel(ScanArg
     for (int v = 0; v < V; ++v) carry[v] = g_last && at.active ? g_last[sc + v] : 0.0f;
   }
   const int64_t sx = q.dir * ldx, sf = q.dir * ldf, sy = q.dir * ldgy;
+  const TileRows<T, V> tx(at, q, ldx), tf(at, q, ldf), ty(at, q, ldgy), tgx(at, q, ldgx), tgf(at, q, ldgf);
+  const int64_t last_tile = j1 > j0 ? j0 + (j1 - j0 - 1) / tile * tile : j0 - tile;
   int turn = 0;
-  const int64_t tiles = j1 > j0 ? (j1 - j0 + tile - 1) / tile : 0;
-  for (int64_t k = tiles - 1; k >= 0; --k, turn ^= 1) {
-    const int64_t jt = j0 + k * tile, j = jt + at.group * kSteps, left = j1 - j;
-    const int n = !at.active || left <= 0 ? 0 : left < kSteps ? (int)left : kSteps;
+  auto one_tile = [&](auto whole, int64_t jt) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    const int64_t j = jt + at.group * kSteps, left = j1 - j;
+    const int n = WHOLE ? kSteps : !at.active || left <= 0 ? 0 : left < kSteps ? (int)left : kSteps;
     Rows<T, V> rx, rf, ry;
-    rx.load(x + q.row(j) * ldx + at.channel, sx, n);
-    rf.load(f + q.row(j) * ldf + at.channel, sf, n);
-    ry.load(gy + q.row(j) * ldgy + at.channel, sy, n);
+    if constexpr (WHOLE) {
+      const int64_t row = q.row(jt);
+      tx.load(x + row * ldx, rx);
+      tf.load(f + row * ldf, rf);
+      ty.load(gy + row * ldgy, ry);
+    } else {
+      rx.load(x + q.row(j) * ldx + at.channel, sx, n);
+      rf.load(f + q.row(j) * ldf + at.channel, sf, n);
+      ry.load(gy + q.row(j) * ldgy + at.channel, sy, n);
+    }
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v)
@@ -452,12 +522,13 @@ __global__ __launch_bounds__(kThreads, 2) void scan_tile_backward_kernel(ScanArg
     for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        ps[i][v] = i < n ? signed_gate((float)rf.r[i][v]) : 0.0f;
+        ps[i][v] = WHOLE || i < n ? signed_gate((float)rf.r[i][v]) : 0.0f;
         xs[i][v] = seen((float)rx.r[i][v], ps[i][v]);
         extend(m[v].A, m[v].G, ps[i][v]);
         m[v].H = step(m[v].H, xs[i][v], ps[i][v]);
       }
     }
+    forget<V>(ps);
 #pragma unroll
     for (int i = kSteps - 1; i >= 0; --i) {
 #pragma unroll
@@ -470,17 +541,24 @@ __global__ __launch_bounds__(kThreads, 2) void scan_tile_backward_kernel(ScanArg
     }
     __syncthreads();
     float c[V];
-    for (int b = 0; b < at.n_groups; ++b) {
-      const int back = at.n_groups - 1 - b;
+#pragma unroll
+    for (int v = 0; v < V; ++v) c[v] = jt == last_tile ? carry[v] : ends[turn ^ 1][at.slot + v];
+    for (int k = 0; k < at.group; ++k) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int i = at.at(b, lanes_v) + v, o = at.at(back, lanes_v) + v;
-        if (b < at.group) h[v] = apply(lds[turn][0][i], lds[turn][1][i], lds[turn][2][i], h[v]);
-        if (back == at.group) c[v] = carry[v];
-        carry[v] = apply(lds[turn][0][o], lds[turn][1][o], lds[turn][3][o], carry[v]);
+        const int i = at.at(k, lanes_v) + v;
+        h[v] = apply(lds[turn][0][i], lds[turn][1][i], lds[turn][2][i], h[v]);
       }
     }
-    if (n > 0) {
+    for (int k = at.n_groups - 1; k > at.group; --k) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int i = at.at(k, lanes_v) + v;
+        c[v] = apply(lds[turn][0][i], lds[turn][1][i], lds[turn][3][i], c[v]);
+      }
+    }
+    if (WHOLE || n > 0) {
+      forget<V>(ps);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
 #pragma unroll
@@ -490,6 +568,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_tile_backward_kernel(ScanArg
           xs[i][v] = above;
         }
       }
+      forget<V>(ps);
       T *ox = gx + q.row(j) * ldgx + at.channel, *of = gf + q.row(j) * ldgf + at.channel;
 #pragma unroll
       for (int i = kSteps - 1; i >= 0; --i) {
@@ -497,16 +576,30 @@ __global__ __launch_bounds__(kThreads, 2) void scan_tile_backward_kernel(ScanArg
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float p = __builtin_fabsf(ps[i][v]), total = c[v] + (float)ry.r[i][v];
-          c[v] = decay(total, ps[i][v]);
-          dx[v] = keeps(ps[i][v]) ? p * total : __builtin_fmaf(ps[i][v], total, total);
-          df[v] = p * (1.0f - p) * total * xs[i][v];
+          const float part = p * total, rest = __builtin_fmaf(-p, total, total);
+          const bool k = keeps(ps[i][v]);
+          dx[v] = k ? part : rest;
+          c[v] = k ? rest : part;
+          df[v] = p * rest * xs[i][v];
         }
-        if (i < n) {
+        if constexpr (WHOLE) {
+          tgx.store(gx + q.row(jt) * ldgx, i, dx);
+          tgf.store(gf + q.row(jt) * ldgf, i, df);
+        } else if (i < n) {
           store_vec<V>(ox + i * (q.dir * ldgx), dx);
           store_vec<V>(of + i * (q.dir * ldgf), df);
         }
       }
     }
+    if (at.group == 0) {  // what goes back into the tile in front
+#pragma unroll
+      for (int v = 0; v < V; ++v) ends[turn][at.slot + v] = carry[v] = c[v];
+    }
+    turn ^= 1;
+  };
+  for (int64_t jt = last_tile; jt >= j0; jt -= tile) {
+    if (a.whole && jt + tile <= j1) one_tile(std::true_type{}, jt);
+    else one_tile(std::false_type{}, jt);
   }
   if (g_h0 && at.chunk == 0 && at.group == 0 && at.active) {
 #pragma unroll
@@ -557,6 +650,12 @@ inline int channels_per_lane(int32_t dtype, int32_t n_channels, std::initializer
   for (int64_t s : strides)
     if (s % 2) return 1;
   return 2;
+}
+
+int32_t whole_tiles(const Plan& p, int32_t n_channels, std::initializer_list<int64_t> strides) {
+  for (int64_t s : strides)
+    if (s > (1 << 20)) return 0;
+  return n_channels == p.per_row * (p.v << p.lane_bits);
 }
 
 // calls f with the element type and the channels per lane
@@ -615,7 +714,7 @@ extern "C" int dc_gated_scan(void* stream, int32_t dtype, const void* d_x, int64
   DC_REQUIRE(aligned(d_y, dtype_size(dtype)), "misaligned pointer");
   const int v = channels_per_lane(dtype, n_channels, {d_x, d_f, d_y}, {x_stride, f_stride, y_stride});
   const Plan p = scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
-  ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0};
+  ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0, whole_tiles(p, n_channels, {x_stride, f_stride, y_stride})};
   const int zeros = zero_rest && n_tokens > 0 ? kZeroBlocks : 0;
   return with_lanes(dtype, v, [&](auto t, auto lanes) {
     using T = decltype(t);
@@ -655,7 +754,7 @@ extern "C" int dc_gated_scan_backward(void* stream, int32_t dtype, const void* d
   DC_REQUIRE(aligned(d_grad_y, dtype_size(dtype)) && aligned(d_grad_x, dtype_size(dtype)) && aligned(d_grad_f, dtype_size(dtype)), "misaligned pointer");
   const int v = channels_per_lane(dtype, n_channels, {d_x, d_f, d_grad_y, d_grad_x, d_grad_f}, {x_stride, f_stride, grad_y_stride, grad_x_stride, grad_f_stride});
   const Plan p = scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
-  ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0};
+  ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0, whole_tiles(p, n_channels, {x_stride, f_stride, grad_y_stride, grad_x_stride, grad_f_stride})};
   const int zeros = zero_rest && n_tokens > 0 ? kZeroBlocks : 0;
   return with_lanes(dtype, v, [&](auto t, auto lanes) {
     using T = decltype(t);
