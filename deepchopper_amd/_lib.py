@@ -113,7 +113,7 @@ _SIGNATURES = {
     "dc_block_norm": (C.c_int, [vp, i32, i32, i64, i32, i32, C.c_float, vp, i64, vp, i64, i32, vp, i64, vp, i32, vp, vp, vp, vp, vp, i64, vp, i64]),
     "dc_block_norm_backward": (C.c_int, [vp, i32, i32, i64, i32, i32, C.c_float, vp, i64, vp, i64, i32, vp, i64, vp, i32, vp, vp, vp, vp, i64, vp, i64,
                                          vp, vp, vp, vp, vp, vp, vp, vp, vp, i64]),
-    "dc_block_norm_workspace": (i64, [i64, i32]),
+    "dc_block_norm_workspace": (i64, [i64, i32, i32]),
 }
 
 _lib = None

@@ -3,7 +3,7 @@
 //
 // HBM-bound: forward 5 row elements of traffic per element (y, gate, residual in; r', n out), backward 8 (y, gate, residual, both
 // gradients in; three out) for 4 row reductions each.  A row stays in registers between its passes: 4 elements a lane and step of 256
-// columns, a row in 2 to 64 lanes of a wavefront up to 256 columns, in one wavefront up to 1 024 (backward 512), in up to 16 of them
+// columns, a row in 2 to 64 lanes of a wavefront up to 256 columns, in one wavefront up to 512 (forward), in up to 16 of them
 // beyond.  Mean and deviation are taken one after the other (no E[x^2] - E[x]^2: a mean far from 0 costs no digits).  Backward, nothing of
 // the forward pass is read back: r', u and both norms' statistics cost less to take again from the inputs than to load.
 // The vectors' gradients: every lane sums its own columns over the rows of its workgroup, the workgroups' sums go to the workspace
@@ -25,6 +25,9 @@ struct NormArgs {
   const float *scale, *post_w, *post_b, *pre_w, *pre_b;
   int32_t lane_bits;  // log2 of the lanes a row takes (6 where it takes whole wavefronts)
   int32_t n_waves;    // wavefronts a row takes
+  // what a team's wavefronts told each other is added up one after the other (forward, two wavefronts: 65 536 x 1000 bf16 153 us against
+  // 200 us) or by the lanes of 16 (backward and more wavefronts: 131 072 x 512 bf16 265 us against 293 us, 32 768 x 2048 292 us against 396 us)
+  int32_t serial;
 };
 
 __device__ __forceinline__ float sigmoid(float x) { return fast_rcp(1.0f + fast_exp2(-x * kLog2e)); }
@@ -43,10 +46,24 @@ struct RawPart {
 // How a row lies in a workgroup: several rows in a wavefront (at most 128 columns), a row in one, a row in several.
 enum Form { kSub, kWave, kTeam };
 
+// columns that wavefront w of a row has (w >= n_waves: 0)
+template <int K>
+__device__ __forceinline__ float columns_of(const NormArgs& a, int w) {
+  int n = 0;
+  if (w >= a.n_waves) return 0.0f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int left = a.width - (w + k * a.n_waves) * 64 * V;
+    n += left < 0 ? 0 : left < 64 * V ? left : 64 * V;
+  }
+  return (float)n;
+}
+
 // Where a thread's columns and rows lie.  Outside kSub the row is the wavefront's, kept in scalar registers.
-template <Form F>
+template <int K, Form F>
 struct Spot {
   int column, step, wave, group, n_groups;  // first column, columns between vectors, row group of the workgroup
+  float inv_own, of_lane;                   // a team's: 1 / columns of this wavefront, columns of wavefront (lane mod 16) of the row
   __device__ __forceinline__ Spot(const NormArgs& a) {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if constexpr (F == kSub) {
@@ -60,20 +77,12 @@ struct Spot {
       n_groups = (int)(blockDim.x >> 6) / per_row;
     }
     step = a.n_waves * 64 * V;
+    if constexpr (F == kTeam) {
+      inv_own = 1.0f / __builtin_fmaxf(columns_of<K>(a, wave - group * a.n_waves), 1.0f);
+      of_lane = columns_of<K>(a, threadIdx.x & 15);
+    }
   }
 };
-
-// columns that wavefront w of a row has
-template <int K>
-__device__ __forceinline__ float columns_of(const NormArgs& a, int w) {
-  int n = 0;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int left = a.width - (w + k * a.n_waves) * 64 * V;
-    n += left < 0 ? 0 : left < 64 * V ? left : 64 * V;
-  }
-  return (float)n;
-}
 
 // the thread's whole vectors of a row, or the single elements of the one that the width cuts
 template <typename T, int K>
@@ -166,19 +175,29 @@ __device__ __forceinline__ void load_weights(const float* w, float other, const 
 // What the wavefronts of a row tell each other, one slot a wavefront, two halves used in turn: one barrier an exchange.
 struct Meeting {
   float2 slot[2][16];
+  // lane l of every 16: what wavefront l of the row said
+  __device__ __forceinline__ float2 of_lane(int turn, int first, int n_waves) const {
+    const int l = threadIdx.x & 15;
+    return l < n_waves ? slot[turn][first + l] : float2{0.0f, 0.0f};
+  }
 };
 
 // Sums over the row of one or two values.
-template <Form F>
-__device__ __forceinline__ float2 row_sums(float x, float y, bool two, const NormArgs& a, const Spot<F>& at, Meeting& m, int& turn) {
+template <int K, Form F>
+__device__ __forceinline__ float2 row_sums(float x, float y, bool two, const NormArgs& a, const Spot<K, F>& at, Meeting& m, int& turn) {
   const int bits = F == kSub ? a.lane_bits : 6;
   float2 s{lanes_sum(x, bits), two ? lanes_sum(y, bits) : 0.0f};
   if constexpr (F == kTeam) {
-    const int first = at.group * a.n_waves;
     if ((threadIdx.x & 63) == 0) m.slot[turn][at.wave] = s;
     __syncthreads();
-    s = m.slot[turn][first];
-    for (int w = 1; w < a.n_waves; ++w) s.x += m.slot[turn][first + w].x, s.y += m.slot[turn][first + w].y;
+    const int first = at.group * a.n_waves;
+    if (a.serial) {
+      s = m.slot[turn][first];
+      for (int w = 1; w < a.n_waves; ++w) s.x += m.slot[turn][first + w].x, s.y += m.slot[turn][first + w].y;
+    } else {
+      s = m.of_lane(turn, first, a.n_waves);
+      s = {lanes_sum(s.x, 4), two ? lanes_sum(s.y, 4) : 0.0f};
+    }
     turn ^= 1;
   }
   return s;
@@ -187,7 +206,7 @@ __device__ __forceinline__ float2 row_sums(float x, float y, bool two, const Nor
 // mean (RMS: 0) and 1 / deviation of a row; elements beyond the width are 0.  The squares are taken about the mean: of the wavefront's own
 // columns first, moved to the row's mean when the wavefronts meet (sum (x - m)^2 = sum (x - m_w)^2 + n_w (m_w - m)^2).
 template <int K, Form F>
-__device__ __forceinline__ float2 row_stats(const Part<K>& p, const NormArgs& a, const Spot<F>& at, Meeting& m, int& turn) {
+__device__ __forceinline__ float2 row_stats(const Part<K>& p, const NormArgs& a, const Spot<K, F>& at, Meeting& m, int& turn) {
   const int bits = F == kSub ? a.lane_bits : 6;
   float mean = 0.0f, q = 0.0f;
   if (a.kind == DC_NORM_LAYER) {
@@ -197,7 +216,7 @@ __device__ __forceinline__ float2 row_stats(const Part<K>& p, const NormArgs& a,
 #pragma unroll
       for (int i = 0; i < V; ++i) s += p.v[k][i];
     s = lanes_sum(s, bits);
-    mean = F == kTeam ? s * fast_rcp(__builtin_fmaxf(columns_of<K>(a, at.wave - at.group * a.n_waves), 1.0f)) : s * a.inv_width;
+    mean = s * (F == kTeam ? at.inv_own : a.inv_width);
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -210,21 +229,31 @@ __device__ __forceinline__ float2 row_stats(const Part<K>& p, const NormArgs& a,
   }
   q = lanes_sum(q, bits);
   if constexpr (F == kTeam) {
-    const int first = at.group * a.n_waves;
     if ((threadIdx.x & 63) == 0) m.slot[turn][at.wave] = {mean, q};
     __syncthreads();
-    q = 0.0f;
-    if (a.kind == DC_NORM_LAYER) {
-      float all = 0.0f;
-      for (int w = 0; w < a.n_waves; ++w) all = __builtin_fmaf(m.slot[turn][first + w].x, columns_of<K>(a, w), all);
-      all *= a.inv_width;
-      for (int w = 0; w < a.n_waves; ++w) {
-        const float2 o = m.slot[turn][first + w];
-        q += __builtin_fmaf((o.x - all) * (o.x - all), columns_of<K>(a, w), o.y);
+    const int first = at.group * a.n_waves;
+    if (a.serial) {
+      q = 0.0f;
+      if (a.kind == DC_NORM_LAYER) {
+        float all = 0.0f;
+        for (int w = 0; w < a.n_waves; ++w) all = __builtin_fmaf(m.slot[turn][first + w].x, columns_of<K>(a, w), all);
+        mean = all * a.inv_width;
+        for (int w = 0; w < a.n_waves; ++w) {
+          const float2 o = m.slot[turn][first + w];
+          q += __builtin_fmaf((o.x - mean) * (o.x - mean), columns_of<K>(a, w), o.y);
+        }
+      } else {
+        for (int w = 0; w < a.n_waves; ++w) q += m.slot[turn][first + w].y;
       }
-      mean = all;
+      turn ^= 1;
+      return {mean, __builtin_amdgcn_rsqf(__builtin_fmaf(q, a.inv_width, a.eps))};
+    }
+    const float2 o = m.of_lane(turn, first, a.n_waves);
+    if (a.kind == DC_NORM_LAYER) {
+      mean = lanes_sum(o.x * at.of_lane, 4) * a.inv_width;
+      q = lanes_sum(__builtin_fmaf((o.x - mean) * (o.x - mean), at.of_lane, o.y), 4);
     } else {
-      for (int w = 0; w < a.n_waves; ++w) q += m.slot[turn][first + w].y;
+      q = lanes_sum(o.y, 4);
     }
     turn ^= 1;
   }
@@ -236,8 +265,8 @@ __device__ __forceinline__ float2 row_stats(const Part<K>& p, const NormArgs& a,
 struct Rows {
   int64_t first, step, n;
   int group;
-  template <Form F>
-  __device__ __forceinline__ Rows(const NormArgs& a, const Spot<F>& at)
+  template <int K, Form F>
+  __device__ __forceinline__ Rows(const NormArgs& a, const Spot<K, F>& at)
       : first((int64_t)blockIdx.x * at.n_groups), step((int64_t)gridDim.x * at.n_groups), n(a.n_rows), group(at.group) {}
   __device__ __forceinline__ int64_t clamped(int64_t f) const { return f + group < n ? f + group : n - 1; }
 };
@@ -247,7 +276,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a, const T
                                                                               int64_t residual_out_stride, T* normed, int64_t normed_stride) {
   __shared__ Meeting meeting;
   int turn = 0;
-  const Spot<F> at(a);
+  const Spot<K, F> at(a);
   const Rows rows(a, at);
   RawPart<T, K> raw_y, raw_g;
   RawPart<R, K> raw_r;
@@ -322,14 +351,14 @@ __global__ __launch_bounds__(THREADS) void block_norm_kernel(NormArgs a, const T
 
 // The gradient g of a normalised row, in place, to that of the row: factor (g - mean(g) - hat mean(g hat)).
 template <int K, Form F>
-__device__ __forceinline__ void norm_back(Part<K>& g, const Part<K>& hat, const NormArgs& a, const Spot<F>& at, float factor, Meeting& m, int& turn) {
+__device__ __forceinline__ void norm_back(Part<K>& g, const Part<K>& hat, const NormArgs& a, const Spot<K, F>& at, float factor, Meeting& m, int& turn) {
   float s = 0.0f, q = 0.0f;
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int i = 0; i < V; ++i) s += g.v[k][i], q = __builtin_fmaf(g.v[k][i], hat.v[k][i], q);
   const bool layer = a.kind == DC_NORM_LAYER;
-  const float2 t = row_sums<F>(q, s, layer, a, at, m, turn);
+  const float2 t = row_sums<K, F>(q, s, layer, a, at, m, turn);
   q = t.x * a.inv_width;
   s = layer ? t.y * a.inv_width : 0.0f;
 #pragma unroll
@@ -340,15 +369,18 @@ __device__ __forceinline__ void norm_back(Part<K>& g, const Part<K>& hat, const 
 
 // Rows as in the forward pass; the workgroup's sums over them, [5][width] in the order scale, post_w, post_b, pre_w, pre_b, go to
 // sums[blockIdx.x].
+// Five workgroups a CU where 16-bit rows leave the registers for it: 262 144 x 256 bf16 320 -> 278 us; with fp32 rows it would spill.
+constexpr int waves_a_simd(int row_bytes, int k, Form f, int threads) { return row_bytes == 2 && k == 1 && f != kSub && threads == 256 ? 5 : 1; }
+
 template <typename T, typename R, int K, Form F, int THREADS>
-__global__ __launch_bounds__(THREADS) void block_norm_backward_kernel(NormArgs a, const T* y, const T* gate, const R* residual,
+__global__ __launch_bounds__(THREADS, waves_a_simd(sizeof(R), K, F, THREADS)) void block_norm_backward_kernel(NormArgs a, const T* y, const T* gate, const R* residual,
                                                                                        const R* g_out, int64_t g_out_stride, const T* g_normed,
                                                                                        int64_t g_normed_stride, T* g_y, T* g_gate, R* g_residual,
                                                                                        float* __restrict__ sums) {
-  extern __shared__ float lds[];  // one vector per row group
+  extern __shared__ __align__(16) float lds[];  // a team's weights, and at the end a vector per row group
   __shared__ Meeting meeting;
   int turn = 0;
-  const Spot<F> at(a);
+  const Spot<K, F> at(a);
   const Rows rows(a, at);
   RawPart<T, K> raw_y, raw_g, raw_n;
   RawPart<R, K> raw_r, raw_o;
@@ -373,13 +405,40 @@ __global__ __launch_bounds__(THREADS) void block_norm_backward_kernel(NormArgs a
     });
   };
   if (rows.first < rows.n) fetch(rows.clamped(rows.first));
-  Part<K> acc[5], sc, w1, b1, w2;
+  // The weights: a team keeps them in LDS (its lanes have no registers to spare), others in registers.
+  Part<K> acc[5], held[F == kTeam ? 1 : 4];
 #pragma unroll
   for (int n = 0; n < 5; ++n) fill(acc[n], 0.0f);
-  load_weights(a.scale, 1.0f, a, at, sc);
-  load_weights(a.post_w, 1.0f, a, at, w1);
-  load_weights(a.post_b, 0.0f, a, at, b1);
-  load_weights(a.pre_w, 1.0f, a, at, w2);
+  const int span = a.n_waves * 64 * V * K;
+  if constexpr (F == kTeam) {
+    for (int c = threadIdx.x; c < span; c += THREADS) {
+      const bool in = c < a.width;
+      lds[c] = in ? a.scale ? a.scale[c] : 1.0f : 0.0f;
+      lds[span + c] = in ? a.post_w ? a.post_w[c] : 1.0f : 0.0f;
+      lds[2 * span + c] = in && a.post_b ? a.post_b[c] : 0.0f;
+      lds[3 * span + c] = in ? a.pre_w ? a.pre_w[c] : 1.0f : 0.0f;
+    }
+    __syncthreads();
+  } else {
+    load_weights(a.scale, 1.0f, a, at, held[0]);
+    load_weights(a.post_w, 1.0f, a, at, held[1]);
+    load_weights(a.post_b, 0.0f, a, at, held[2]);
+    load_weights(a.pre_w, 1.0f, a, at, held[3]);
+  }
+  enum { kScale, kPostW, kPostB, kPreW };
+  auto weights = [&](int n) {
+    if constexpr (F == kTeam) {
+      Part<K> p;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const float4 q = *reinterpret_cast<const float4*>(lds + n * span + at.column + k * at.step);
+        p.v[k][0] = q.x, p.v[k][1] = q.y, p.v[k][2] = q.z, p.v[k][3] = q.w;
+      }
+      return p;
+    } else {
+      return held[n];
+    }
+  };
   for (int64_t f = rows.first; f < rows.n; f += rows.step) {
     const int64_t row = f + at.group;
     const bool live = row < rows.n;
@@ -403,6 +462,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_backward_kernel(NormArgs a
 #pragma unroll
           for (int i = 0; i < V; ++i) hat.v[k][i] = (hat.v[k][i] - st.x) * st.y;
       }
+      const Part<K> sc = weights(kScale), w1 = weights(kPostW), b1 = weights(kPostB);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -414,6 +474,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_backward_kernel(NormArgs a
     }
     if (g_normed) {  // r becomes the normalised r', t the gradient of r' through the norm
       const float2 st2 = row_stats<K, F>(r, a, at, meeting, turn);
+      const Part<K> w2 = weights(kPreW);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -436,6 +497,7 @@ __global__ __launch_bounds__(THREADS) void block_norm_backward_kernel(NormArgs a
     }
     r = t;  // the gradient of the residual
     if (y) {
+    const Part<K> sc = weights(kScale), w1 = weights(kPostW), b1 = weights(kPostB);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -509,7 +571,9 @@ __global__ __launch_bounds__(1024) void block_norm_sums_kernel(const float* __re
   }
 }
 
-// How many lanes, wavefronts and vectors a row takes.  Backward: 5 sums a column besides the row, so half as many columns a lane.
+// How many lanes, wavefronts and vectors a row takes: lanes of a wavefront up to 256 columns, then (forward) two vectors a lane, then up to
+// 16 wavefronts.  Backward there are 5 sums a column besides the row: one vector a lane while 16 wavefronts suffice (two would leave 2
+// instead of 4 or 5 workgroups a CU: 131 072 x 512 bf16 548 us against 265 us).
 struct RowPlan {
   int lane_bits, n_waves, k, threads;
 };
@@ -521,13 +585,7 @@ RowPlan row_plan(int32_t width, bool backward) {
     while ((1 << p.lane_bits) < lanes) ++p.lane_bits;
     return p;
   }
-#ifndef BW_MOST
-#define BW_MOST 1
-#endif
-#ifndef FW_MOST
-#define FW_MOST 2
-#endif
-  const int most = backward ? BW_MOST : FW_MOST;
+  const int most = backward ? 1 : 2;
   while (p.k < most && width > 64 * V * p.k) p.k *= 2;
   while (width > 64 * V * p.k * p.n_waves && p.n_waves < 16) p.n_waves *= 2;
   if (width > 64 * V * p.k * p.n_waves) p.k *= 2;
@@ -536,11 +594,12 @@ RowPlan row_plan(int32_t width, bool backward) {
 }
 
 // workgroups of the backward pass = parts of the vectors' sums
-int parts_of(int64_t n_rows, int32_t width) {
+int parts_of(int64_t n_rows, int32_t width, int32_t residual_dtype) {
   const RowPlan p = row_plan(width, true);
   const int groups = p.n_waves > 1 ? p.threads / 64 / p.n_waves : p.threads >> p.lane_bits;
-  int64_t most = (1 << 21) / width;  // at most 40 MB of them, ...
-  most = most > 1024 ? 1024 : most < 256 ? 256 : most;
+  int64_t most = (1 << 21) / width;  // at most 40 MB of them, but one for every CU
+  const int full = residual_dtype != DC_DTYPE_F32 && (p.n_waves > 1 || p.lane_bits == 6) && p.threads == 256 ? 1280 : 1024;  // (what runs at once)
+  most = most > full ? full : most < 256 ? 256 : most;
   const int64_t need = (n_rows + groups - 1) / groups;
   return (int)(need < most ? need : most);
 }
@@ -584,8 +643,8 @@ int with_row(int32_t dtype, int32_t residual_dtype, const RowPlan& p, F&& f) {
 }  // namespace
 }  // namespace dc
 
-extern "C" int64_t dc_block_norm_workspace(int64_t n_rows, int32_t width) {
-  return n_rows > 0 && width > 0 ? (int64_t)dc::parts_of(n_rows, width) * 5 * width * 4 : 0;
+extern "C" int64_t dc_block_norm_workspace(int64_t n_rows, int32_t width, int32_t residual_dtype) {
+  return n_rows > 0 && width > 0 ? (int64_t)dc::parts_of(n_rows, width, residual_dtype) * 5 * width * 4 : 0;
 }
 
 extern "C" int dc_block_norm(void* stream, int32_t dtype, int32_t residual_dtype, int64_t n_rows, int32_t width, int32_t kind, float eps,
@@ -601,7 +660,7 @@ extern "C" int dc_block_norm(void* stream, int32_t dtype, int32_t residual_dtype
   if (n_rows == 0 || (!d_residual_out && !d_normed)) return DC_OK;
   const RowPlan p = row_plan(width, false);
   const NormArgs a{n_rows, width, kind, gate_act, post_norm, eps, 1.0f / width, y_stride, gate_stride, residual_stride,
-                   d_scale, d_post_w, d_post_b, d_pre_w, d_pre_b, p.lane_bits, p.n_waves};
+                   d_scale, d_post_w, d_post_b, d_pre_w, d_pre_b, p.lane_bits, p.n_waves, p.n_waves == 2};
   const int groups = p.n_waves > 1 ? p.threads / 64 / p.n_waves : p.threads >> p.lane_bits;
   const int64_t need = (n_rows + groups - 1) / groups;
   const int grid = (int)(need < 4096 ? need : 4096);
@@ -628,20 +687,21 @@ extern "C" int dc_block_norm_backward(void* stream, int32_t dtype, int32_t resid
   DC_REQUIRE(aligned(d_grad_residual_out, dtype_size(residual_dtype)) && aligned(d_grad_residual, dtype_size(residual_dtype)) &&
                  aligned(d_grad_normed, dtype_size(dtype)) && aligned(d_grad_y, dtype_size(dtype)) && aligned(d_grad_gate, dtype_size(dtype)),
              "misaligned pointer");
-  DC_REQUIRE(workspace_bytes >= dc_block_norm_workspace(n_rows, width) && (n_rows == 0 || d_workspace) && aligned(d_workspace, 16), "workspace too small");
+  DC_REQUIRE(workspace_bytes >= dc_block_norm_workspace(n_rows, width, residual_dtype) && (n_rows == 0 || d_workspace) && aligned(d_workspace, 16), "workspace too small");
   const RowPlan p = row_plan(width, true);
   const NormArgs a{n_rows, width, kind, gate_act, post_norm, eps, 1.0f / width, y_stride, gate_stride, residual_stride,
-                   d_scale, d_post_w, d_post_b, d_pre_w, nullptr, p.lane_bits, p.n_waves};
+                   d_scale, d_post_w, d_post_b, d_pre_w, nullptr, p.lane_bits, p.n_waves, 0};
   const int groups = p.n_waves > 1 ? p.threads / 64 / p.n_waves : p.threads >> p.lane_bits;
-  const int grid = parts_of(n_rows, width);
+  const int grid = parts_of(n_rows, width, residual_dtype);
   const bool any = d_grad_scale || d_grad_post_w || d_grad_post_b || d_grad_pre_w || d_grad_pre_b;
   return with_row(dtype, residual_dtype, p, [&](auto t, auto r, auto k, auto form, auto threads) {
     using T = decltype(t);
     using R = decltype(r);
     if (grid > 0) {
       auto kernel = block_norm_backward_kernel<T, R, decltype(k)::value, decltype(form)::value, decltype(threads)::value>;
-      DC_SET_MAX_SMEM_ONCE_PER_DEVICE(kernel, DC_MAX_NORM_WIDTH * 4);
-      kernel<<<dim3(grid), dim3(p.threads), groups * width * 4, as_stream(stream)>>>(
+      DC_SET_MAX_SMEM_ONCE_PER_DEVICE(kernel, DC_MAX_NORM_WIDTH * 16);
+      const int held = p.n_waves > 1 ? 4 * p.n_waves * 64 * V * p.k : 0, floats = held > groups * width ? held : groups * width;
+      kernel<<<dim3(grid), dim3(p.threads), floats * 4, as_stream(stream)>>>(
           a, (const T*)d_y, (const T*)d_gate, (const R*)d_residual, (const R*)d_grad_residual_out, grad_residual_out_stride,
           (const T*)d_grad_normed, grad_normed_stride, (T*)d_grad_y, (T*)d_grad_gate, (R*)d_grad_residual, any ? (float*)d_workspace : nullptr);
       DC_LAUNCH_CHECK();

@@ -480,7 +480,7 @@ def block_norm_backward(y: torch.Tensor | None, residual: torch.Tensor | None = 
          "grad_scale": grad(scale) if y is not None else None, "grad_post_weight": grad(post_weight) if normed else None,
          "grad_post_bias": grad(post_bias) if normed else None, "grad_pre_weight": grad(pre_weight), "grad_pre_bias": grad(pre_bias)}
     L = _lib.lib()
-    nb = L.dc_block_norm_workspace(n, w)
+    nb = L.dc_block_norm_workspace(n, w, _DTYPES[res_dtype])
     ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
     with _on(dev):
         _lib.check(L.dc_block_norm_backward(

@@ -508,7 +508,7 @@ int dc_block_norm_backward(void* stream, int32_t dtype, int32_t residual_dtype, 
                            int64_t grad_normed_stride, void* d_grad_y, void* d_grad_gate, void* d_grad_residual,
                            float* d_grad_scale, float* d_grad_post_w, float* d_grad_post_b, float* d_grad_pre_w,
                            float* d_grad_pre_b, void* d_workspace, int64_t workspace_bytes);
-int64_t dc_block_norm_workspace(int64_t n_rows, int32_t width);
+int64_t dc_block_norm_workspace(int64_t n_rows, int32_t width, int32_t residual_dtype);
 
 #ifdef __cplusplus
 }

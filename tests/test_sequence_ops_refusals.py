@@ -97,9 +97,9 @@ def test_block_norm_refusals(L):
     back = lambda ws=P, nb=1 << 30, n=4: L.dc_block_norm_backward(  # noqa: E731
         None, 0, 0, n, 8, 0, 1e-5, P, 8, None, 0, 0, P, 8, None, 1, None, None, None, P, 8, P, 8, P, None, P, None, None, None, None, None, ws, nb)
     refused(L, back(ws=None), "workspace")
-    refused(L, back(nb=L.dc_block_norm_workspace(4, 8) - 1), "workspace")
+    refused(L, back(nb=L.dc_block_norm_workspace(4, 8, 0) - 1), "workspace")
     refused(L, back(ws=C.c_void_p(4100)), "workspace")
-    assert L.dc_block_norm_workspace(0, 8) == 0 and L.dc_block_norm_workspace(1 << 40, 8192) < 1 << 31
+    assert L.dc_block_norm_workspace(0, 8, 0) == 0 and L.dc_block_norm_workspace(1 << 40, 8192, 2) < 1 << 31
     assert norm(L, n=0) == 0 and norm(L, out=None, normed=None) == 0
 
 
