@@ -21,7 +21,7 @@ import torch
 
 from . import ops
 from .fastq import decode_names
-from .tokenizer import DEFAULT_MAX_LENGTH, PAD_TOKEN_ID, check_read_status, encode_ids_int8
+from .tokenizer import DEFAULT_MAX_LENGTH, IGNORE_INDEX, PAD_TOKEN_ID, check_read_status, encode_ids_int8
 
 
 @dataclass
@@ -219,8 +219,9 @@ class PredictPipeline:
         return res
 
     # ---- host-facing convenience -----------------------------------------------------------
-    def predict_reads(self, ids: list[str], seqs: list[bytes], quals: list[bytes], *, reference_padding: bool = False):
-        """Returns one dict per read: id, labels (int8), smoothed labels, intervals, keep segments."""
+    def predict_reads(self, ids: list[str], seqs: list[bytes], quals: list[bytes], *, reference_padding: bool = False, want_scores: bool = False):
+        """Returns one dict per read: id, labels (int8), smoothed labels, intervals, keep segments; with `want_scores` also, per
+        base, `log_prob` (float32: of the predicted label) and `entropy` (of the two classes, in nats): how sure the model was."""
         for i, s, q in zip(ids, seqs, quals):
             if not i or not s or not q:
                 raise ValueError("Incomplete FASTQ record")  # only_fq.py:38-40
@@ -238,6 +239,9 @@ class PredictPipeline:
         pred, smooth = sm["pred"].cpu().numpy(), sm["smooth"].cpu().numpy()
         iv, niv = sm["intervals"].cpu().numpy(), sm["n_intervals"].cpu().numpy()
         kp, nkp = sm["keep"].cpu().numpy(), sm["n_keep"].cpu().numpy()
+        if want_scores:  # (labels: 0 on bases, -100 on padding and [SEP], which are skipped; the first alternative is the prediction)
+            sc = ops.token_logprobs(res["logits"], res["tok"]["labels"], n_top=1, ignore_index=IGNORE_INDEX)
+            log_prob, entropy = sc["top_logprob"][..., 0].cpu().numpy(), sc["entropy"].cpu().numpy()
         out = []
         for r, rid in enumerate(ids):
             out.append({
@@ -248,6 +252,9 @@ class PredictPipeline:
                 "keep": [tuple(x) for x in kp[r, : nkp[r]].tolist()],
                 "is_truncated": bool(status[r] & 1),
             })
+            if want_scores:
+                bases = slice(int(res["first"][r]), int(res["first"][r]) + int(res["n_tokens"][r]) - 1)
+                out[-1].update(log_prob=log_prob[r, bases].copy(), entropy=entropy[r, bases].copy())
         return out, res
 
     # ---- streaming: FASTQ chunks -> labels / intervals, host I/O overlapped with GPU work ---------------

@@ -686,3 +686,29 @@ def test_wrappers_refuse(env):
         with pytest.raises(DeepChopperHipError):
             call()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("padding", [False, True])
+def test_predict_reads_scores(env, padding):
+    """`predict_reads(want_scores=True)`: the log probability of every base's predicted label and the entropy, of the logits of that call."""
+    torch, ops = env
+    from deepchopper_amd import synth
+    from deepchopper_amd.model import DeepChopper
+    from deepchopper_amd.predict import PredictPipeline
+    from deepchopper_amd.weights import synthetic_state_dict
+    from oracle import sequence_ref as ref
+
+    pipe = PredictPipeline(DeepChopper.from_state_dict(synthetic_state_dict(0)))
+    rng = np.random.default_rng(45)
+    reads = [synth.synth_reads_fixed(1, int(n), seed=int(n)) for n in rng.integers(30, 400, 5)]
+    ids, seqs, quals = [f"r{i}" for i in range(5)], [r[0][0].tobytes() for r in reads], [r[1][0].tobytes() for r in reads]
+    plain, _ = pipe.predict_reads(ids, seqs, quals, reference_padding=padding)
+    out, res = pipe.predict_reads(ids, seqs, quals, reference_padding=padding, want_scores=True)
+    logits = res["logits"].cpu().numpy()
+    for i, (o, p) in enumerate(zip(out, plain)):
+        assert "log_prob" not in p and o["intervals"] == p["intervals"] and np.array_equal(o["prediction"], p["prediction"])
+        first, n = int(res["first"][i]), len(seqs[i])
+        want, bound = ref.token_logprobs(logits[i, first:first + n], n_top=1)
+        assert o["log_prob"].shape == o["entropy"].shape == (n,) and np.array_equal(want["top_ids"][:, 0], o["prediction"])
+        for name, w, b in (("log_prob", want["top_logprob"][:, 0], bound["top_logprob"][:, 0]), ("entropy", want["entropy"], bound["entropy"])):
+            assert (np.abs(o[name] - w) <= b + HALF_STEP["float32"] * np.abs(w) + TINY["float32"]).all(), name
