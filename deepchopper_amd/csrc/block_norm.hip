@@ -411,7 +411,7 @@ __global__ __launch_bounds__(THREADS, waves_a_simd(sizeof(R), K, F, THREADS)) vo
   for (int n = 0; n < 5; ++n) fill(acc[n], 0.0f);
   const int span = a.n_waves * 64 * V * K;
   if constexpr (F == kTeam) {
-    for (int c = threadIdx.x; c < span; c += THREADS) {
+    for (int c = threadIdx.x; c < span; c += blockDim.x) {
       const bool in = c < a.width;
       lds[c] = in ? a.scale ? a.scale[c] : 1.0f : 0.0f;
       lds[span + c] = in ? a.post_w ? a.post_w[c] : 1.0f : 0.0f;
@@ -585,11 +585,10 @@ RowPlan row_plan(int32_t width, bool backward) {
     while ((1 << p.lane_bits) < lanes) ++p.lane_bits;
     return p;
   }
-  const int most = backward ? 1 : 2;
-  while (p.k < most && width > 64 * V * p.k) p.k *= 2;
-  while (width > 64 * V * p.k * p.n_waves && p.n_waves < 16) p.n_waves *= 2;
-  if (width > 64 * V * p.k * p.n_waves) p.k *= 2;
-  if (p.n_waves > 4) p.threads = 64 * p.n_waves;
+  const int one = (width + 64 * V - 1) / (64 * V), two = (width + 128 * V - 1) / (128 * V);  // wavefronts with one or two vectors a lane
+  p.k = backward ? one > 16 ? 2 : 1 : one <= 16 && 5 * one < 8 * two ? 1 : 2;                // (forward: two, unless a fifth of them would be idle)
+  p.n_waves = p.k == 1 ? one : two;
+  p.threads = p.n_waves <= 2 ? 256 : 64 * p.n_waves;
   return p;
 }
 
@@ -598,7 +597,7 @@ int parts_of(int64_t n_rows, int32_t width, int32_t residual_dtype) {
   const RowPlan p = row_plan(width, true);
   const int groups = p.n_waves > 1 ? p.threads / 64 / p.n_waves : p.threads >> p.lane_bits;
   int64_t most = (1 << 21) / width;  // at most 40 MB of them, but one for every CU
-  const int full = residual_dtype != DC_DTYPE_F32 && (p.n_waves > 1 || p.lane_bits == 6) && p.threads == 256 ? 1280 : 1024;  // (what runs at once)
+  const int full = residual_dtype != DC_DTYPE_F32 && (p.n_waves > 1 || p.lane_bits == 6) && p.n_waves <= 4 ? 1280 : 1024;  // (what runs at once)
   most = most > full ? full : most < 256 ? 256 : most;
   const int64_t need = (n_rows + groups - 1) / groups;
   return (int)(need < most ? need : most);

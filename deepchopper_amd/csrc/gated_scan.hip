@@ -122,8 +122,10 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_kernel(ScanArgs a, con
                                                                  const float* h0, T* __restrict__ y, int64_t ldy, float* h_last) {
   if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, y, ldy, nullptr, 0);
   const int per_seq = (a.n_channels + kWalkThreads * V - 1) / (kWalkThreads * V);
-  const int s = blockIdx.x / per_seq, c = (blockIdx.x % per_seq * kWalkThreads + threadIdx.x) * V;
+  const int s = blockIdx.x / per_seq;
+  int c = (blockIdx.x % per_seq * kWalkThreads + threadIdx.x) * V;
   if (c >= a.n_channels) return;
+  if (c + V > a.n_channels) c = a.n_channels - V;
   const Seq q(a, s);
   const int64_t sc = (int64_t)s * a.n_channels + c;
   float h[V];
@@ -157,8 +159,10 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_backward_kernel(ScanAr
   if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, gx, ldgx, gf, ldgf);
   __shared__ float above[kShort][kWalkThreads * V];  // h_(t-1) - x_t
   const int per_seq = (a.n_channels + kWalkThreads * V - 1) / (kWalkThreads * V);
-  const int s = blockIdx.x / per_seq, c = (blockIdx.x % per_seq * kWalkThreads + threadIdx.x) * V;
+  const int s = blockIdx.x / per_seq;
+  int c = (blockIdx.x % per_seq * kWalkThreads + threadIdx.x) * V;
   if (c >= a.n_channels) return;
+  if (c + V > a.n_channels) c = a.n_channels - V;
   const Seq q(a, s);
   const int64_t sc = (int64_t)s * a.n_channels + c;
   const int n = (int)q.len;
@@ -217,6 +221,7 @@ struct Place {
     s = (int)blockIdx.x / per_row / a.n_chunks;
     slot = lane * V;
     active = channel < a.n_channels;
+    if (active && channel + V > a.n_channels) channel = a.n_channels - V;  // (an odd number of channels: the last pair overlaps)
   }
   __device__ __forceinline__ int at(int grp, int lanes_v) const { return grp * lanes_v + slot; }
 };
@@ -230,7 +235,7 @@ struct Rows {
     for (int i = 0; i < kSteps; ++i) {
       if (i < n) {
         if constexpr (V == 1) r[i][0] = p[i * ld];
-        else r[i] = *reinterpret_cast<const vec_t<T, V>*>(p + i * ld);
+        else r[i] = *reinterpret_cast<const typename loose_vec<T, V>::type*>(p + i * ld);
       } else {
         r[i] = vec_t<T, V>(0);
       }
@@ -255,7 +260,7 @@ struct TileRows {
     for (int i = 0; i < kSteps; ++i) {
       const char* p = reinterpret_cast<const char*>(tile + first + i * per_step) + lane;
       if constexpr (V == 1) to.r[i][0] = *reinterpret_cast<const T*>(p);
-      else to.r[i] = *reinterpret_cast<const vec_t<T, V>*>(p);
+      else to.r[i] = *reinterpret_cast<const typename loose_vec<T, V>::type*>(p);
     }
   }
   __device__ __forceinline__ void store(T* tile, int i, const float (&v)[V]) const {
@@ -624,11 +629,10 @@ Plan scan_plan(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max
   const int64_t rows = (int64_t)n_seqs * p.per_row;
   int64_t all = (n_tokens + tile - 1) / tile * p.per_row;  // tiles of the whole call, if its sequences fill them
   if (all > rows * tiles) all = rows * tiles;
-  // a workgroup's fair share of tiles, over four workgroups a CU, and at least four of them
+  // a workgroup's fair share of tiles, over four workgroups a CU
   int64_t share = (all + 1023) / 1024;
-  if (share < 4) share = 4;
   p.n_chunks = 1;
-  if (tiles > 2 * share) {
+  if (tiles > 2 * share && tiles > 6) {  // (a second kernel takes as long as a few tiles)
     int64_t c = (tiles + share - 1) / share;
     const int64_t most = rows > 0 ? (1 << 18) / rows : 1;  // short sequences have as many chunks as the longest: mostly empty workgroups
     if (c > 1024) c = 1024;
@@ -642,14 +646,10 @@ Plan scan_plan(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max
   return p;
 }
 
-// V channels per lane: two where 16-bit rows are even and aligned to both
-inline int channels_per_lane(int32_t dtype, int32_t n_channels, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> strides) {
-  if (dtype == DC_DTYPE_F32 || n_channels % 2) return 1;
-  for (const void* p : ptrs)
-    if (!aligned(p, 4)) return 1;
-  for (int64_t s : strides)
-    if (s % 2) return 1;
-  return 2;
+// Channels per lane: two of 16 bits.  Of an odd number, the last lane takes the last two, one of them its neighbour's as well: both compute
+// and write the same bits (a state kept in place, h_last = h0, could be overwritten by the one before the other has read it: one a lane then).
+inline int channels_per_lane(int32_t dtype, int32_t n_channels, bool in_place) {
+  return dtype == DC_DTYPE_F32 || n_channels == 1 || (in_place && n_channels % 2) ? 1 : 2;
 }
 
 int32_t whole_tiles(const Plan& p, int32_t n_channels, std::initializer_list<int64_t> strides) {
@@ -712,7 +712,7 @@ extern "C" int dc_gated_scan(void* stream, int32_t dtype, const void* d_x, int64
   DC_REQUIRE(n_tokens == 0 || d_y, "null pointer");
   DC_REQUIRE(y_stride >= n_channels, "rows of the output overlap");
   DC_REQUIRE(aligned(d_y, dtype_size(dtype)), "misaligned pointer");
-  const int v = channels_per_lane(dtype, n_channels, {d_x, d_f, d_y}, {x_stride, f_stride, y_stride});
+  const int v = channels_per_lane(dtype, n_channels, d_h0 && d_h0 == d_h_last);
   const Plan p = scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
   ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0, whole_tiles(p, n_channels, {x_stride, f_stride, y_stride})};
   const int zeros = zero_rest && n_tokens > 0 ? kZeroBlocks : 0;
@@ -752,7 +752,7 @@ extern "C" int dc_gated_scan_backward(void* stream, int32_t dtype, const void* d
   DC_REQUIRE(grad_y_stride >= 0, "negative stride");
   DC_REQUIRE(grad_x_stride >= n_channels && grad_f_stride >= n_channels, "rows of an output overlap");
   DC_REQUIRE(aligned(d_grad_y, dtype_size(dtype)) && aligned(d_grad_x, dtype_size(dtype)) && aligned(d_grad_f, dtype_size(dtype)), "misaligned pointer");
-  const int v = channels_per_lane(dtype, n_channels, {d_x, d_f, d_grad_y, d_grad_x, d_grad_f}, {x_stride, f_stride, grad_y_stride, grad_x_stride, grad_f_stride});
+  const int v = channels_per_lane(dtype, n_channels, d_grad_h0 && d_grad_h0 == d_grad_h_last);
   const Plan p = scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
   ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0, whole_tiles(p, n_channels, {x_stride, f_stride, grad_y_stride, grad_x_stride, grad_f_stride})};
   const int zeros = zero_rest && n_tokens > 0 ? kZeroBlocks : 0;

@@ -3,7 +3,7 @@
 // HBM-bound: a row is read once (backward: read once, written once).  With m the row's maximum, S = sum exp(z - m) and
 // U = sum exp(z - m) (z - m):   log p_j = (z_j - m) - log S    H = log S - U / S    dz_j = p_j (-g - h (log p_j + H)) + g [j = t]
 //
-// Up to 512 classes a row lives in the registers of 1 to 64 lanes (4 neighbouring classes a lane; 8 beyond 256), forward and backward:
+// Up to 512 classes a row lives in the registers of 1 to 32 lanes (2 to 16 classes a lane), forward and backward:
 // the two-class logits of a predict batch are one lane a row.  There S is summed without its largest term's 1 and log S = log1p(S - 1), so a
 // row that is sure of its class keeps the digits of -log p.
 // Beyond, a wavefront walks the row (or, where there are few rows, one of up to 64 slices of it, joined by a second kernel) in pieces of
@@ -111,7 +111,7 @@ __device__ __forceinline__ RowStats few_stats(const Few<E>& f, int bits) {
     const float d = f.z[i] - ref, e = fast_exp2(d * kLog2e);
     ones += d == 0.0f ? 1.0f : 0.0f;
     s += d == 0.0f ? 0.0f : e;
-    u += e > 0.0f ? e * d : 0.0f;
+    u = __builtin_fmaf(e, __builtin_fmaxf(d, -150.0f), u);  // (e is 0 there, and 0 x -inf is not wanted)
   }
   s = lanes_sum(s, bits);
   ones = lanes_sum(ones, bits);
@@ -123,7 +123,7 @@ __device__ __forceinline__ RowStats few_stats(const Few<E>& f, int bits) {
 }
 
 // ONE: a row is one lane's (bits = 0, known to the compiler)
-template <typename T, int E, bool ONE>
+template <typename T, int E, bool ONE, bool TOP>
 __global__ __launch_bounds__(256) void few_classes_kernel(const T* __restrict__ logits, int64_t n_rows, int32_t n, int64_t ld, int32_t lane_bits, Tokens tok,
                                                           int32_t n_top, float* __restrict__ logprob, float* __restrict__ entropy,
                                                           float* __restrict__ stats, int32_t* __restrict__ top_ids, float* __restrict__ top_logprob) {
@@ -155,28 +155,60 @@ __global__ __launch_bounds__(256) void few_classes_kernel(const T* __restrict__ 
       if (entropy) entropy[i] = r.entropy;
       if (stats) stats[3 * i] = r.m, stats[3 * i + 1] = r.log_sum, stats[3 * i + 2] = r.entropy;
     }
-    uint32_t used = 0;
-    for (int k = 0; k < n_top; ++k) {
-      float lp = 0.0f;
-      int id = -1;
-      if (!skip) {
-        uint32_t key = 0;
-        int at = 0;
+    if constexpr (!TOP) continue;
+    if (skip) {
+      for (int k = lane; k < n_top; k += 1 << bits) top_ids[i * n_top + k] = -1, top_logprob[i * n_top + k] = 0.0f;
+      continue;
+    }
+    uint32_t key[E];  // 0: no class
+#pragma unroll
+    for (int q = 0; q < E; ++q) key[q] = f.c[q] < n ? order_key(f.z[q]) : 0;
+    if constexpr (E <= 4) {
+      if (3 * n_top > 2 << bits) {  // (a lane's classes are counted in two thirds of the time of a round below)
+        // Every class counts how many are better -- of an equal logit, those of lower classes -- and writes itself to that place.  Classes go
+        // by (vector, lane, place in the vector).
+        constexpr int W = Few<E>::W;
+        int rank[E];
 #pragma unroll
         for (int q = 0; q < E; ++q) {
-          const uint32_t o = f.c[q] < n && !(used >> q & 1) ? order_key(f.z[q]) : 0;
-          if (o > key) key = o, at = q;
-        }
-        const uint32_t best = lanes_reduce_u32(key, bits, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-        int c = 0;
+          rank[q] = 0;
 #pragma unroll
-        for (int q = 0; q < E; ++q)
-          if (q == at) c = f.c[q];
-        id = (int)lanes_reduce_u32(key == best ? (uint32_t)c : 0x7fffffffu, bits, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
-        if (key == best && c == id) used |= 1u << at;
-        lp = log_prob(r, key_value(best));
+          for (int o = 0; o < E; ++o) rank[q] += o < q ? key[o] >= key[q] : key[o] > key[q];
+        }
+        if constexpr (!ONE) {
+          for (int l = 0; l < 1 << bits; ++l) {
+            uint32_t least[E];  // what a class of lane l in the same vector has to exceed
+#pragma unroll
+            for (int q = 0; q < E; ++q) least[q] = key[q] - (l < lane ? 1 : 0);
+#pragma unroll
+            for (int o = 0; o < E; ++o) {
+              uint32_t other = (uint32_t)__shfl((int)key[o], l, 1 << bits);
+              if (l == lane) other = 0;
+#pragma unroll
+              for (int q = 0; q < E; ++q) rank[q] += other > (o / W < q / W ? key[q] - 1 : o / W > q / W ? key[q] : least[q]);
+            }
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < E; ++q) {
+          if (key[q] != 0 && rank[q] < n_top)
+            top_ids[i * n_top + rank[q]] = f.c[q], top_logprob[i * n_top + rank[q]] = log_prob(r, key_value(key[q]));
+        }
+        continue;
       }
-      if (lane == 0) top_ids[i * n_top + k] = id, top_logprob[i * n_top + k] = lp;
+    }
+    for (int k = 0; k < n_top; ++k) {  // the best one that is left, n_top times
+      uint32_t mine = key[0];
+      int c = f.c[0];
+#pragma unroll
+      for (int q = 1; q < E; ++q)
+        if (key[q] > mine) mine = key[q], c = f.c[q];
+      const uint32_t best = lanes_reduce_u32(mine, bits, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+      const int id = (int)lanes_reduce_u32(mine == best ? (uint32_t)c : 0x7fffffffu, bits, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+#pragma unroll
+      for (int q = 0; q < E; ++q)
+        if (f.c[q] == id) key[q] = 0;
+      if (lane == 0) top_ids[i * n_top + k] = id, top_logprob[i * n_top + k] = log_prob(r, key_value(best));
     }
   }
 }
@@ -588,10 +620,12 @@ int slices_of(int64_t n_rows, int32_t n_classes) {
   return (int)(s > kMaxSlices ? kMaxSlices : s < 1 ? 1 : s);
 }
 
-// lanes a row takes up to 512 classes, as a power of two
+// Up to 512 classes: classes a lane and lanes a row, as a power of two.  4 neighbouring classes a lane and up to 16 lanes; then more of
+// them a lane, so that four (two) rows share a wavefront's reductions.
+int few_classes_a_lane(int32_t n_classes) { return n_classes <= 2 ? 2 : n_classes <= 64 ? 4 : n_classes <= 128 ? 8 : 16; }
 int lane_bits_of(int32_t n_classes) {
   int bits = 0;
-  while (n_classes > 4 << bits && bits < 6) ++bits;
+  while (n_classes > few_classes_a_lane(n_classes) << bits) ++bits;
   return bits;
 }
 
@@ -601,7 +635,11 @@ int with_few(int32_t dtype, int32_t n_classes, F&& f) {
   return with_dtype(dtype, [&](auto t) {
     if (n_classes <= 2) return f(t, std::integral_constant<int, 2>{}, std::true_type{});
     if (n_classes <= 4) return f(t, std::integral_constant<int, 4>{}, std::true_type{});
-    return n_classes <= 256 ? f(t, std::integral_constant<int, 4>{}, std::false_type{}) : f(t, std::integral_constant<int, 8>{}, std::false_type{});
+    switch (few_classes_a_lane(n_classes)) {
+      case 4: return f(t, std::integral_constant<int, 4>{}, std::false_type{});
+      case 8: return f(t, std::integral_constant<int, 8>{}, std::false_type{});
+      default: return f(t, std::integral_constant<int, 16>{}, std::false_type{});
+    }
   });
 }
 
@@ -641,7 +679,8 @@ extern "C" int dc_token_logprobs(void* stream, const void* d_logits, int32_t dty
     const int bits = lane_bits_of(n_classes);
     return with_few(dtype, n_classes, [&](auto t, auto e, auto one) {
       using T = decltype(t);
-      few_classes_kernel<T, decltype(e)::value, decltype(one)::value><<<dim3(grid_of((n_rows + (256 >> bits) - 1) / (256 >> bits))), dim3(256), 0, as_stream(stream)>>>(
+      auto kernel = n_top > 0 ? few_classes_kernel<T, decltype(e)::value, decltype(one)::value, true> : few_classes_kernel<T, decltype(e)::value, decltype(one)::value, false>;
+      kernel<<<dim3(grid_of((n_rows + (256 >> bits) - 1) / (256 >> bits))), dim3(256), 0, as_stream(stream)>>>(
           (const T*)d_logits, n_rows, n_classes, row_stride, bits, tok, n_top, d_logprob, d_entropy, d_stats, d_top_ids, d_top_logprob);
       DC_LAUNCH_CHECK();
       return DC_OK;

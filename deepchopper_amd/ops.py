@@ -394,6 +394,9 @@ def gated_scan_backward(x: torch.Tensor, f: torch.Tensor, saved: torch.Tensor, g
     return {"grad_x": gx, "grad_f": gf, "grad_h0": gh}
 
 
+_NORM_VECTORS = ("grad_scale", "grad_post_weight", "grad_post_bias", "grad_pre_weight", "grad_pre_bias")
+
+
 def _norm_ref(y, residual) -> torch.Tensor:
     ref = y if y is not None else residual
     _need(ref is not None, "block_norm: a block's output or a residual is required")
@@ -472,22 +475,22 @@ def block_norm_backward(y: torch.Tensor | None, residual: torch.Tensor | None = 
     qw = _like(dev, "pre_weight", pre_weight, one, torch.float32)
     _like(dev, "pre_bias", pre_bias, one, torch.float32)
 
-    def grad(like, dt=torch.float32):
-        return None if like is None else torch.empty(like.shape, dtype=dt, device=device)
-
     normed = post and y is not None
-    g = {"grad_y": grad(y, act_dtype), "grad_gate": grad(gate, act_dtype), "grad_residual": grad(residual, res_dtype),
-         "grad_scale": grad(scale) if y is not None else None, "grad_post_weight": grad(post_weight) if normed else None,
-         "grad_post_bias": grad(post_bias) if normed else None, "grad_pre_weight": grad(pre_weight), "grad_pre_bias": grad(pre_bias)}
+    sums = torch.empty((5, w), dtype=torch.float32, device=device).unbind()
+    wanted = (y is not None and scale is not None, normed and post_weight is not None, normed and post_bias is not None, pre_weight is not None,
+              pre_bias is not None)
+    vectors = [t if want else None for t, want in zip(sums, wanted)]
+    gy = None if y is None else torch.empty(shape, dtype=act_dtype, device=device)
+    gg = None if gate is None else torch.empty(shape, dtype=act_dtype, device=device)
+    gr = None if residual is None else torch.empty(shape, dtype=res_dtype, device=device)
     L = _lib.lib()
     nb = L.dc_block_norm_workspace(n, w, _DTYPES[res_dtype])
     ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
     with _on(dev):
         _lib.check(L.dc_block_norm_backward(
             _stream_of(dev), _DTYPES[act_dtype], _DTYPES[res_dtype], n, w, k, eps, yp, ys, gp, gs, act, rp, rs, sc, int(post), pw, pb, qw, grp, grs,
-            gnp, gns, *(_address(g[m]) for m in ("grad_y", "grad_gate", "grad_residual", "grad_scale", "grad_post_weight", "grad_post_bias",
-                                                 "grad_pre_weight", "grad_pre_bias")), _address(ws), nb))
-    return g
+            gnp, gns, _address(gy), _address(gg), _address(gr), *map(_address, vectors), _address(ws), nb))
+    return {"grad_y": gy, "grad_gate": gg, "grad_residual": gr, **dict(zip(_NORM_VECTORS, vectors))}
 
 
 # ------------------------------------------------------------------------------------------
