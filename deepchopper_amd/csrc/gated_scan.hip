@@ -114,6 +114,13 @@ __device__ void zero_rest(const ScanArgs& a, int block, T* y, int64_t ldy, T* y2
   }
 }
 
+// Of an odd number of channels the last lane takes the last two and writes only the second: the first is its neighbour's.
+template <int V, typename T>
+__device__ __forceinline__ void store_channels(T* p, const float (&v)[V], bool second) {
+  if (V == 2 && second) p[V - 1] = (T)v[V - 1];
+  else store_vec<V>(p, v);
+}
+
 // ---- sequences of at most kShort tokens: a thread per V channels ---------------------------------------------------------------
 constexpr int kWalkThreads = 64;
 
@@ -125,7 +132,8 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_kernel(ScanArgs a, con
   const int s = blockIdx.x / per_seq;
   int c = (blockIdx.x % per_seq * kWalkThreads + threadIdx.x) * V;
   if (c >= a.n_channels) return;
-  if (c + V > a.n_channels) c = a.n_channels - V;
+  const bool second = c + V > a.n_channels;
+  if (second) --c;
   const Seq q(a, s);
   const int64_t sc = (int64_t)s * a.n_channels + c;
   float h[V];
@@ -142,11 +150,12 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_kernel(ScanArgs a, con
       const float ps = signed_gate(fv[v]);
       h[v] = step(h[v], seen(xv[v], ps), ps);
     }
-    store_vec<V>(y + t * ldy + c, h);
+    store_channels<V>(y + t * ldy + c, h, second);
   }
   if (h_last) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) h_last[sc + v] = q.ok ? h[v] : __builtin_nanf("");
+    for (int v = 0; v < V; ++v) h[v] = q.ok ? h[v] : __builtin_nanf("");
+    store_channels<V>(h_last + sc, h, second);
   }
 }
 
@@ -162,7 +171,8 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_backward_kernel(ScanAr
   const int s = blockIdx.x / per_seq;
   int c = (blockIdx.x % per_seq * kWalkThreads + threadIdx.x) * V;
   if (c >= a.n_channels) return;
-  if (c + V > a.n_channels) c = a.n_channels - V;
+  const bool second = c + V > a.n_channels;
+  if (second) --c;
   const Seq q(a, s);
   const int64_t sc = (int64_t)s * a.n_channels + c;
   const int n = (int)q.len;
@@ -196,12 +206,13 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_backward_kernel(ScanAr
       g[v] = keeps(ps) ? rest : part;
       of[v] = p * rest * above[j][threadIdx.x * V + v];
     }
-    store_vec<V>(gx + t * ldgx + c, ox);
-    store_vec<V>(gf + t * ldgf + c, of);
+    store_channels<V>(gx + t * ldgx + c, ox, second);
+    store_channels<V>(gf + t * ldgf + c, of, second);
   }
   if (g_h0) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) g_h0[sc + v] = q.ok ? g[v] : __builtin_nanf("");
+    for (int v = 0; v < V; ++v) g[v] = q.ok ? g[v] : __builtin_nanf("");
+    store_channels<V>(g_h0 + sc, g, second);
   }
 }
 
@@ -210,7 +221,7 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_backward_kernel(ScanAr
 template <int V>
 struct Place {
   int s, chunk, group, n_groups, channel, slot;  // slot: of this thread's channels in a group's row of LDS
-  bool active;
+  bool active, second;                           // second: see store_channels
   __device__ __forceinline__ Place(const ScanArgs& a) {
     const int lanes = 1 << a.lane_bits, per_row = (a.n_channels + lanes * V - 1) / (lanes * V);
     const int lane = threadIdx.x & (lanes - 1);
@@ -221,7 +232,8 @@ struct Place {
     s = (int)blockIdx.x / per_row / a.n_chunks;
     slot = lane * V;
     active = channel < a.n_channels;
-    if (active && channel + V > a.n_channels) channel = a.n_channels - V;  // (an odd number of channels: the last pair overlaps)
+    second = active && channel + V > a.n_channels;
+    if (second) --channel;
   }
   __device__ __forceinline__ int at(int grp, int lanes_v) const { return grp * lanes_v + slot; }
 };
@@ -288,8 +300,7 @@ __global__ __launch_bounds__(kThreads) void scan_map_kernel(ScanArgs a, const T*
   const int lanes_v = V << a.lane_bits;
   const int64_t j0 = at.chunk * a.chunk, part = a.chunk / at.n_groups;
   if (at.chunk == 0 && at.active && at.group == 0) {
-#pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int v = at.second ? 1 : 0; v < V; ++v)
       maps[start_at(a, at.s, at.channel + v)] = start ? start[(int64_t)at.s * a.n_channels + at.channel + v] : 0.0f;
   }
   if (j0 >= q.len) return;
@@ -325,8 +336,7 @@ __global__ __launch_bounds__(kThreads) void scan_map_kernel(ScanArgs a, const T*
   }
   __syncthreads();
   if (at.group != 0 || !at.active) return;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
+  for (int v = at.second ? 1 : 0; v < V; ++v) {
     Span all = identity_span();
     for (int k = 0; k < at.n_groups; ++k) {
       const int i = at.at(BACK ? at.n_groups - 1 - k : k, lanes_v) + v;
@@ -444,8 +454,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, cons
     if (WHOLE || n > 0) {
       forget<V>(ps);
       if (saved && j % kTile == 0 && j > 0) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) saved[q.row(j) / kTile * a.n_channels + at.channel + v] = h[v];
+        store_channels<V>(saved + (q.row(j) / kTile * a.n_channels + at.channel), h, at.second);
       }
       T* out = y + q.row(j) * ldy + at.channel;
 #pragma unroll
@@ -453,7 +462,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, cons
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = step(h[v], xs[i][v], ps[i][v]);
         if constexpr (WHOLE) ty.store(y + q.row(jt) * ldy, i, h);
-        else if (i < n) store_vec<V>(out + i * sy, h);
+        else if (i < n) store_channels<V>(out + i * sy, h, at.second);
       }
     }
     if (last_group) {  // the state behind the tile, for the next one
@@ -468,7 +477,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, cons
   for (; jt < j1; jt += tile) one_tile(std::false_type{}, jt);
   if (h_last && last_group && at.active && j1 == q.len) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) h_last[sc + v] = q.ok ? carry[v] : __builtin_nanf("");
+    for (int v = 0; v < V; ++v) carry[v] = q.ok ? carry[v] : __builtin_nanf("");
+    store_channels<V>(h_last + sc, carry, at.second);
   }
 }
 
@@ -591,8 +601,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_backward_kernel(ScanArg
           tgx.store(gx + q.row(jt) * ldgx, i, dx);
           tgf.store(gf + q.row(jt) * ldgf, i, df);
         } else if (i < n) {
-          store_vec<V>(ox + i * (q.dir * ldgx), dx);
-          store_vec<V>(of + i * (q.dir * ldgf), df);
+          store_channels<V>(ox + i * (q.dir * ldgx), dx, at.second);
+          store_channels<V>(of + i * (q.dir * ldgf), df, at.second);
         }
       }
     }
@@ -608,7 +618,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_backward_kernel(ScanArg
   }
   if (g_h0 && at.chunk == 0 && at.group == 0 && at.active) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) g_h0[sc + v] = q.ok ? carry[v] : __builtin_nanf("");
+    for (int v = 0; v < V; ++v) carry[v] = q.ok ? carry[v] : __builtin_nanf("");
+    store_channels<V>(g_h0 + sc, carry, at.second);
   }
 }
 
@@ -630,9 +641,9 @@ Plan scan_plan(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max
   int64_t all = (n_tokens + tile - 1) / tile * p.per_row;  // tiles of the whole call, if its sequences fill them
   if (all > rows * tiles) all = rows * tiles;
   // a workgroup's fair share of tiles, over four workgroups a CU
-  int64_t share = (all + 1023) / 1024;
+  int64_t share = all > 1024 ? (all + 1023) / 1024 : 1;
   p.n_chunks = 1;
-  if (tiles > 2 * share && tiles > 6) {  // (a second kernel takes as long as a few tiles)
+  if (n_tokens > 0 && tiles > 2 * share && tiles > 6) {  // (a second kernel takes as long as a few tiles)
     int64_t c = (tiles + share - 1) / share;
     const int64_t most = rows > 0 ? (1 << 18) / rows : 1;  // short sequences have as many chunks as the longest: mostly empty workgroups
     if (c > 1024) c = 1024;
@@ -646,11 +657,8 @@ Plan scan_plan(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max
   return p;
 }
 
-// Channels per lane: two of 16 bits.  Of an odd number, the last lane takes the last two, one of them its neighbour's as well: both compute
-// and write the same bits (a state kept in place, h_last = h0, could be overwritten by the one before the other has read it: one a lane then).
-inline int channels_per_lane(int32_t dtype, int32_t n_channels, bool in_place) {
-  return dtype == DC_DTYPE_F32 || n_channels == 1 || (in_place && n_channels % 2) ? 1 : 2;
-}
+// Channels per lane: two of 16 bits.
+inline int channels_per_lane(int32_t dtype, int32_t n_channels) { return dtype == DC_DTYPE_F32 || n_channels == 1 ? 1 : 2; }
 
 int32_t whole_tiles(const Plan& p, int32_t n_channels, std::initializer_list<int64_t> strides) {
   for (int64_t s : strides)
@@ -712,7 +720,7 @@ extern "C" int dc_gated_scan(void* stream, int32_t dtype, const void* d_x, int64
   DC_REQUIRE(n_tokens == 0 || d_y, "null pointer");
   DC_REQUIRE(y_stride >= n_channels, "rows of the output overlap");
   DC_REQUIRE(aligned(d_y, dtype_size(dtype)), "misaligned pointer");
-  const int v = channels_per_lane(dtype, n_channels, d_h0 && d_h0 == d_h_last);
+  const int v = channels_per_lane(dtype, n_channels);
   const Plan p = scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
   ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0, whole_tiles(p, n_channels, {x_stride, f_stride, y_stride})};
   const int zeros = zero_rest && n_tokens > 0 ? kZeroBlocks : 0;
@@ -752,7 +760,7 @@ extern "C" int dc_gated_scan_backward(void* stream, int32_t dtype, const void* d
   DC_REQUIRE(grad_y_stride >= 0, "negative stride");
   DC_REQUIRE(grad_x_stride >= n_channels && grad_f_stride >= n_channels, "rows of an output overlap");
   DC_REQUIRE(aligned(d_grad_y, dtype_size(dtype)) && aligned(d_grad_x, dtype_size(dtype)) && aligned(d_grad_f, dtype_size(dtype)), "misaligned pointer");
-  const int v = channels_per_lane(dtype, n_channels, d_grad_h0 && d_grad_h0 == d_grad_h_last);
+  const int v = channels_per_lane(dtype, n_channels);
   const Plan p = scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
   ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0, whole_tiles(p, n_channels, {x_stride, f_stride, grad_y_stride, grad_x_stride, grad_f_stride})};
   const int zeros = zero_rest && n_tokens > 0 ? kZeroBlocks : 0;

@@ -646,6 +646,7 @@ int with_few(int32_t dtype, int32_t n_classes, F&& f) {
 int check_logits(const void* logits, int32_t dtype, int64_t n_rows, int32_t n_classes, int64_t row_stride, const void* tokens, int32_t token_type) {
   DC_REQUIRE(dtype_ok(dtype), "unknown element type");
   DC_REQUIRE(n_rows >= 0 && n_classes >= 1, "negative size");
+  DC_REQUIRE(n_classes <= 1 << 30, "more than 2^30 classes");
   DC_REQUIRE(n_rows == 0 || logits, "null pointer");
   DC_REQUIRE(row_stride >= 0, "negative stride");
   DC_REQUIRE(token_type >= DC_TOKENS_I8 && token_type <= DC_TOKENS_I64, "unknown token type");

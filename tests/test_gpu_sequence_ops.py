@@ -180,8 +180,14 @@ def test_gated_scan_tokens_outside_the_offsets(env):
     assert torch.equal(kept["y"][30:300], made["y"][30:300])
     for t, v in ((out, 7.0), (made["y"], 0.0), (g["grad_x"], 0.0), (g["grad_f"], 0.0)):
         assert (t[:30] == v).all() and (t[300:] == v).all()
-    none = ops.gated_scan(x, f, offsets=torch.zeros(1, dtype=torch.int64, device="cuda"), max_len=0)
-    assert (none["y"] == 0).all() and none["h_last"].shape == (0, c)
+    for max_len in (0, 5000):
+        none = ops.gated_scan(x, f, offsets=torch.zeros(1, dtype=torch.int64, device="cuda"), max_len=max_len)
+        assert (none["y"] == 0).all() and none["h_last"].shape == (0, c)
+        h0 = make(torch, gen, 3, c)
+        empty = ops.gated_scan(x[:0], f[:0], offsets=torch.zeros(4, dtype=torch.int64, device="cuda"), max_len=max_len, h0=h0, save=True)
+        assert torch.equal(empty["h_last"], h0)
+        back = ops.gated_scan_backward(x[:0], f[:0], empty["saved"], gy[:0], grad_h_last=h0, offsets=torch.zeros(4, dtype=torch.int64, device="cuda"), max_len=max_len)
+        assert torch.equal(back["grad_h0"], h0)
 
 
 def test_gated_scan_streams_token_by_token(env):
@@ -197,6 +203,39 @@ def test_gated_scan_streams_token_by_token(env):
         assert r["h_last"] is h
         assert (r["y"][:, 0] - whole["y"][:, t]).abs().max() < 2e-6 and torch.equal(r["y"][:, 0], h)
     assert (h - whole["h_last"]).abs().max() < 2e-6  # 150 steps: at most 150 x 6 x 2^-24 x 1 / 50 of memory apart
+
+
+@pytest.mark.parametrize("n,c,dtype", [(3000, 33, "bfloat16"), (300, 129, "float16"), (5, 7, "bfloat16"), (3000, 64, "float32")])
+def test_gated_scan_state_kept_in_place(env, n, c, dtype):
+    """h_last = h0, over chunks, tiles and single tokens, odd channels included: what a state of its own gives."""
+    torch, ops = env
+    gen = torch.Generator().manual_seed(16)
+    x, f = make(torch, gen, 2, n, c, dtype=dtype), make(torch, gen, 2, n, c, dtype=dtype, shift=4.0)
+    h0 = make(torch, gen, 2, c)
+    want = ops.gated_scan(x, f, h0=h0)
+    for _ in range(3):
+        h = h0.clone()
+        got = ops.gated_scan(x, f, h0=h, h_last=h)
+        assert got["h_last"] is h
+        # (one channel a lane or two: the same steps, so the same bits)
+        assert torch.equal(h, want["h_last"]) and torch.equal(got["y"], want["y"])
+
+
+def test_gated_scan_strides_beyond_a_tile_offset(env):
+    """Rows more than 2^20 elements apart: whole tiles go the checked way too."""
+    from oracle import sequence_ref as ref
+
+    torch, ops = env
+    gen = torch.Generator().manual_seed(17)
+    n, c = 200, 64
+    wide = torch.empty((n, (1 << 20) + 8), dtype=torch.bfloat16, device="cuda")
+    x, f = wide[:, :c], wide[:, c:2 * c]
+    x.copy_(torch.randn((n, c), generator=gen))
+    f.copy_(torch.randn((n, c), generator=gen) + 1)
+    for reverse in (False, True):
+        r = ops.gated_scan(x, f, offsets=torch.tensor([0, n]).cuda(), max_len=n, reverse=reverse)
+        want, bound = ref.gated_scan(host(x), host(f), [(0, n)], reverse=reverse)
+        check("y", r["y"], want["y"], bound["y"])
 
 
 def test_gated_scan_refuses_bad_sequences_on_the_device(env):

@@ -30,6 +30,7 @@ def test_token_logprobs_refusals(L):
     refused(L, logprobs(L, ttype=4), "token type")
     refused(L, logprobs(L, n=-1), "negative size")
     refused(L, logprobs(L, classes=0), "negative size")
+    refused(L, logprobs(L, classes=(1 << 30) + 1, stride=1 << 31), "2^30")
     refused(L, logprobs(L, stride=-8), "negative stride")
     refused(L, logprobs(L, z=ODD, dtype=1), "misaligned")
     refused(L, logprobs(L, tok=ODD), "misaligned")
@@ -70,6 +71,12 @@ def test_gated_scan_refusals(L):
     refused(L, back(gf=None), "null pointer")
     refused(L, back(gxs=5), "overlap")
     refused(L, back(gx=ODD), "misaligned")
+    # nothing to do, whatever the longest sequence might be
+    assert scan(L, seqs=0, longest=100000) == 0 and scan(L, seqs=0, n=0, x=None, f=None, y=None, longest=100000) == 0
+    assert L.dc_gated_scan_workspace(100, 8, 0, 100000) == 0 and L.dc_gated_scan_workspace(0, 8, 3, 100000) == 0
+    # one long sequence needs the maps of its chunks, 16 tokens a step at a time nothing
+    assert L.dc_gated_scan_workspace(100000, 64, 1, 100000) > 0 and L.dc_gated_scan_workspace(1600, 64, 100, 16) == 0
+    refused(L, scan(L, n=100000, c=8, seqs=1, longest=100000), "workspace")
     assert L.dc_gated_scan_saved(0, 8) == 0 and L.dc_gated_scan_saved(1, 8) == 8 and L.dc_gated_scan_saved(65, 8) == 16
     assert L.dc_gated_scan_saved(1 << 33, 256) == 1 << 35
 
