@@ -256,6 +256,11 @@ def _rows(dev: int, name: str, t: torch.Tensor | None, shape: torch.Size | None 
     return t.data_ptr(), dims[-1][1] if dims else size[-1]
 
 
+def _new_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A dense tensor of `t`'s shape and device (`empty_like` takes half the time of `empty`)."""
+    return torch.empty_like(t) if t.dtype is dtype and t.is_contiguous() else torch.empty(t.shape, dtype=dtype, device=t.device)
+
+
 def _address(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -282,7 +287,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     n = logits.numel() // n_classes if n_classes else 0
     tok, kind = _tokens(dev, tokens, lead)
     logprob = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=device)
-    entropy = torch.empty(lead, dtype=torch.float32, device=device) if want_entropy else None
+    entropy = None
+    if want_entropy:
+        entropy = torch.empty_like(logprob) if logprob is not None else torch.empty(lead, dtype=torch.float32, device=device)
     stats = torch.empty((n, 3), dtype=torch.float32, device=device) if save and n_classes >= STATS_FROM else None
     ids = torch.empty((*lead, n_top), dtype=torch.int32, device=device) if n_top > 0 else None
     top = torch.empty((*lead, n_top), dtype=torch.float32, device=device) if n_top > 0 else None
@@ -307,7 +314,7 @@ def token_logprobs_backward(logits: torch.Tensor, tokens: torch.Tensor | None, s
     st = _like(dev, "stats", stats, (n, 3), torch.float32)
     gl = _like(dev, "grad_logprob", grad_logprob, lead, torch.float32)
     gh = _like(dev, "grad_entropy", grad_entropy, lead, torch.float32)
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    out = _new_like(logits, logits.dtype)
     with _on(dev):
         _lib.check(_lib.lib().dc_token_logprobs_backward(_stream_of(dev), ptr, _DTYPES[logits.dtype], n, n_classes, stride, tok, kind, ignore_index, st,
                                                          gl, gh, out.data_ptr(), n_classes))
@@ -353,10 +360,10 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, *, offsets: torch.Tensor | None
     h0p = _like(dev, "h0", h0, (seqs, c), torch.float32)
     zero_rest = out is None and offsets is not None  # (dense sequences cover every token)
     if out is None:
-        out = (torch.empty if begin is None else torch.zeros)(shape, dtype=dtype, device=device)
+        out = _new_like(x, dtype) if begin is None else torch.zeros(shape, dtype=dtype, device=device)
     yp, ys = _rows(dev, "out", out, shape, dtype)
     if h_last is None:
-        h_last = torch.empty((seqs, c), dtype=torch.float32, device=device)
+        h_last = torch.empty_like(h0) if h0 is not None else torch.empty((seqs, c), dtype=torch.float32, device=device)
     hp = _like(dev, "h_last", h_last, (seqs, c), torch.float32)
     L = _lib.lib()
     saved = torch.empty(L.dc_gated_scan_saved(n, c), dtype=torch.float32, device=device) if save else None
@@ -383,8 +390,10 @@ def gated_scan_backward(x: torch.Tensor, f: torch.Tensor, saved: torch.Tensor, g
     h0p = _like(dev, "h0", h0, (seqs, c), torch.float32)
     glp = _like(dev, "grad_h_last", grad_h_last, (seqs, c), torch.float32)
     sp = _like(dev, "saved", saved, (L.dc_gated_scan_saved(n, c),), torch.float32)
-    make = torch.empty if begin is None else torch.zeros
-    gx, gf = make(shape, dtype=dtype, device=device), make(shape, dtype=dtype, device=device)
+    if begin is None:
+        gx, gf = _new_like(x, dtype), _new_like(f, dtype)
+    else:
+        gx, gf = torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
     gh = torch.empty((seqs, c), dtype=torch.float32, device=device)
     nb = L.dc_gated_scan_workspace(n, c, seqs, longest)
     ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
@@ -436,9 +445,9 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None = None, gat
     pw, pb = _like(dev, "post_weight", post_weight, one, torch.float32), _like(dev, "post_bias", post_bias, one, torch.float32)
     qw, qb = _like(dev, "pre_weight", pre_weight, one, torch.float32), _like(dev, "pre_bias", pre_bias, one, torch.float32)
     if out is None and y is not None:
-        out = torch.empty(shape, dtype=res_dtype, device=device)
+        out = _new_like(residual if residual is not None else y, res_dtype)
     op, os_ = _rows(dev, "out", out, shape, res_dtype)
-    normed = torch.empty(shape, dtype=act_dtype, device=device) if pre else None
+    normed = _new_like(ref, act_dtype) if pre else None
     with _on(dev):
         _lib.check(_lib.lib().dc_block_norm(
             _stream_of(dev), _DTYPES[act_dtype], _DTYPES[res_dtype], ref.numel() // w if w else 0, w, k, eps, yp, ys, gp, gs, act, rp, rs, sc,
@@ -480,9 +489,9 @@ def block_norm_backward(y: torch.Tensor | None, residual: torch.Tensor | None = 
     wanted = (y is not None and scale is not None, normed and post_weight is not None, normed and post_bias is not None, pre_weight is not None,
               pre_bias is not None)
     vectors = [t if want else None for t, want in zip(sums, wanted)]
-    gy = None if y is None else torch.empty(shape, dtype=act_dtype, device=device)
-    gg = None if gate is None else torch.empty(shape, dtype=act_dtype, device=device)
-    gr = None if residual is None else torch.empty(shape, dtype=res_dtype, device=device)
+    gy = None if y is None else _new_like(y, act_dtype)
+    gg = None if gate is None else _new_like(gate, act_dtype)
+    gr = None if residual is None else _new_like(residual, res_dtype)
     L = _lib.lib()
     nb = L.dc_block_norm_workspace(n, w, _DTYPES[res_dtype])
     ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
