@@ -7,11 +7,13 @@
 // drift by 2^-25 a step).  A span of steps is the map h -> H + A h; it carries both A and G = 1 - A and is applied with the
 // smaller of them, for the same reason.  Weights below 2^-126 are 0.
 //
-// Form.  HBM-bound: 3 elements of traffic per element forward, 5 backward, about 30 and 50 vector operations.  Lanes run along the
+// Form.  HBM-bound: 3 elements of traffic per element forward, 5 backward, about 35 and 50 vector operations.  Lanes run along the
 // channels (a row of 64 lanes is 256 contiguous bytes), time is divided: a workgroup's 8 wavefronts take 8 consecutive tokens each of
 // a 64-token tile (narrow batches: 16 or 32 lanes a row and 32 or 16 such groups), keep them in registers, pass each other their
 // maps through LDS and run the steps again from the state they then know.  Where sequences and channels alone do not fill the chip,
 // a sequence is divided into chunks: a first kernel reads each chunk for its map alone, the second starts from the composed maps.
+// Measured (a large copy: 4.7 TB/s): 1 024 sequences of 500 - 1 500 x 256 bf16 339 us = 4.6 TB/s; 255 of 20 - 4 001 x 768 fp16 forward 588 us =
+// 4.0 TB/s, backward 960 us = 4.1 TB/s (vector work, 80 - 85 % busy); one of 100 001 x 256 fp32 45 + 61 us and 40 + 97 us backward.
 #include <initializer_list>
 #include <type_traits>
 

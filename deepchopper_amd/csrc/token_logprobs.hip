@@ -11,6 +11,9 @@
 // Top alternatives of a walk: the n-th largest of the lanes' (or quads') maxima bounds the n-th largest class from below, so one comparison
 // a class against that bound leaves a few candidates, which are collected in LDS and ranked by counting; the bound only rises from
 // there on.  Ties go to the lower class throughout: candidates are ordered by (logit, class).
+// Measured (a large copy: 4.7 TB/s): 2 050 048 x 2 fp32 with one alternative 12.5 us (47 MB); 4 096 x 100 003 bf16 forward 188 us = 4.4 TB/s,
+// backward 272 us = 6 TB/s; 16 384 x 4 096 bf16 with four alternatives 50 us (vector work, 22 operations a class); 5 x 50 257 fp16 with
+// twenty 9.3 + 6.7 us (latency).
 #include <type_traits>
 
 #include "elem_io.h"
