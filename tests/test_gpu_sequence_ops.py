@@ -751,3 +751,82 @@ def test_predict_reads_scores(env, padding):
         assert o["log_prob"].shape == o["entropy"].shape == (n,) and np.array_equal(want["top_ids"][:, 0], o["prediction"])
         for name, w, b in (("log_prob", want["top_logprob"][:, 0], bound["top_logprob"][:, 0]), ("entropy", want["entropy"], bound["entropy"])):
             assert (np.abs(o[name] - w) <= b + HALF_STEP["float32"] * np.abs(w) + TINY["float32"]).all(), name
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype,c", [("float32", 5), ("bfloat16", 131), ("float16", 64)])
+def test_gated_scan_short_sequences_at_begin_and_end(env, reverse, dtype, c):
+    """Up to 16 tokens of each row, gaps and sequences that break the contract among them: the token-by-token form."""
+    torch, ops = env
+    from oracle import sequence_ref as ref
+
+    gen = torch.Generator().manual_seed(46)
+    n = 120
+    x, f, gy = (make(torch, gen, n, c, dtype=dtype) for _ in range(3))
+    ranges = [(100, 112), (3, 3), (7, 8), (20, 36), (60, 59), (110, 121), (40, 57)]
+    good = [0, 1, 2, 3]
+    b, e = (torch.tensor([r[i] for r in ranges]).cuda() for i in (0, 1))
+    r = ops.gated_scan(x, f, begin=b, end=e, max_len=16, reverse=reverse, save=True)
+    g = ops.gated_scan_backward(x, f, r["saved"], gy, begin=b, end=e, max_len=16, reverse=reverse)
+    want, bound = ref.gated_scan(host(x), host(f), [ranges[i] for i in good], None, reverse, host(gy))
+    covered = torch.from_numpy(~np.isnan(want["y"][:, 0])).cuda()
+    for name, t in {"y": r["y"], "grad_x": g["grad_x"], "grad_f": g["grad_f"]}.items():
+        check(name, t[covered], want[name][covered.cpu().numpy()], bound[name][covered.cpu().numpy()])
+        assert (t[~covered] == 0).all()
+    for name, t in {"h_last": r["h_last"], "grad_h0": g["grad_h0"]}.items():
+        check(name, t[good], want[name], bound[name])
+        assert torch.isnan(t[4:]).all()
+
+
+def test_gated_scan_of_padded_rows_in_a_graph(env):
+    """begin / end inside a captured graph: the gaps are cleared at every replay."""
+    torch, ops = env
+    gen = torch.Generator().manual_seed(47)
+    x, f = make(torch, gen, 300, 32), make(torch, gen, 300, 32)
+    b, e = torch.tensor([10, 150]).cuda(), torch.tensor([90, 300]).cuda()
+    ops.gated_scan(x, f, begin=b, end=e, max_len=150)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.gated_scan(x, f, begin=b, end=e, max_len=150)
+    for turn in range(4):
+        x.copy_(torch.randn((300, 32), generator=gen))
+        b.copy_(torch.tensor([10 + turn, 150 + turn]))
+        out["y"].fill_(9.0)
+        g.replay()
+        torch.cuda.synchronize()
+        want = ops.gated_scan(x, f, begin=b, end=e, max_len=150)
+        assert torch.equal(out["y"], want["y"]) and torch.equal(out["h_last"], want["h_last"]), turn
+
+
+def test_block_norm_first_norm_in_another_type(env):
+    """The first norm of a model: an fp32 stream in, 16-bit activations out, and back."""
+    torch, ops = env
+    from oracle import sequence_ref as ref
+
+    gen = torch.Generator().manual_seed(48)
+    for w in (64, 300):
+        r, gr, gn = make(torch, gen, 40, w), make(torch, gen, 40, w), make(torch, gen, 40, w, dtype="bfloat16")
+        q = make(torch, gen, w, shift=1.0, scale=0.1)
+        got = ops.block_norm(None, r, pre_weight=q, dtype=torch.bfloat16)
+        back = ops.block_norm_backward(None, r, grad_residual=gr, grad_normed=gn, pre_weight=q)
+        want, bound = ref.block_norm(None, host(r), None, kind="layer", act="identity", pre_weight=host(q), grad_residual=host(gr), grad_normed=host(gn))
+        assert got["normed"].dtype == torch.bfloat16 and back["grad_residual"].dtype == torch.float32
+        check("normed", got["normed"], want["normed"], bound["normed"])
+        for k in ("grad_residual", "grad_pre_weight"):
+            check(k, back[k], want[k], bound[k])
+
+
+@pytest.mark.parametrize("classes", [2, 40, 300, 513, 9001])
+def test_token_logprobs_gradient_in_place_of_the_logits(env, classes):
+    """The C entry takes d_logits as d_grad_logits."""
+    torch, ops = env
+    from deepchopper_amd import _lib
+
+    gen = torch.Generator().manual_seed(49)
+    z, t, gl, gh = logit_inputs(torch, gen, 33, classes, "float16")
+    r = ops.token_logprobs(z, t, save=True)
+    want = ops.token_logprobs_backward(z, t, r["stats"], gl, gh)
+    _lib.check(_lib.lib().dc_token_logprobs_backward(torch.cuda.current_stream().cuda_stream, z.data_ptr(), 1, 33, classes, classes, t.data_ptr(), 3, -100,
+                                                     None if r["stats"] is None else r["stats"].data_ptr(), gl.data_ptr(), gh.data_ptr(), z.data_ptr(), classes))
+    assert torch.equal(z, want)
