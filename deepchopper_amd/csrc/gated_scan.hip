@@ -13,7 +13,7 @@
 // maps through LDS and run the steps again from the state they then know.  Where sequences and channels alone do not fill the chip,
 // a sequence is divided into chunks: a first kernel reads each chunk for its map alone, the second starts from the composed maps.
 // Measured (a large copy: 4.7 TB/s): 1 024 sequences of 500 - 1 500 x 256 bf16 339 us = 4.6 TB/s; 255 of 20 - 4 001 x 768 fp16 forward 588 us =
-// 4.0 TB/s, backward 960 us = 4.1 TB/s (vector work, 80 - 85 % busy); one of 100 001 x 256 fp32 45 + 61 us and 40 + 97 us backward.
+// 4.0 TB/s, backward 960 us = 4.1 TB/s (vector work, 80 - 85 % busy); one of 100 001 x 256 fp32 44 + 56 us and 39 + 91 us backward.
 #include <initializer_list>
 #include <type_traits>
 
@@ -635,6 +635,7 @@ struct Plan {
 Plan scan_plan(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max_len, int v) {
   Plan p;
   p.v = v;
+  if (max_len > n_tokens) max_len = n_tokens;  // (a longer sequence does not fit)
   const int lanes_needed = (n_channels + v - 1) / v;
   p.lane_bits = lanes_needed > 32 ? 6 : lanes_needed > 16 ? 5 : 4;
   p.per_row = (lanes_needed + (1 << p.lane_bits) - 1) >> p.lane_bits;
@@ -642,20 +643,22 @@ Plan scan_plan(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max
   const int64_t rows = (int64_t)n_seqs * p.per_row;
   int64_t all = (n_tokens + tile - 1) / tile * p.per_row;  // tiles of the whole call, if its sequences fill them
   if (all > rows * tiles) all = rows * tiles;
-  // a workgroup's fair share of tiles, over four workgroups a CU
-  int64_t share = all > 1024 ? (all + 1023) / 1024 : 1;
+  // A workgroup's fair share of tiles: of sequences as long as the longest, over the two workgroups a CU that run at once (one of 100 001 x
+  // 256 bf16 64 + 89 us against 77 + 105 us with twice as many); of unequal ones over four (8 of 8 - 19 k x 274 109 + 157 us against
+  // 123 + 178 us with half as many).
+  const int64_t target = 10 * all >= 9 * rows * tiles ? 512 : 1024;
+  const int64_t share = all > target ? (all + target - 1) / target : 1;
   p.n_chunks = 1;
+  int64_t each = tiles;  // tiles of a chunk
   if (n_tokens > 0 && tiles > 2 * share && tiles > 6) {  // (a second kernel takes as long as a few tiles)
     int64_t c = (tiles + share - 1) / share;
     const int64_t most = rows > 0 ? (1 << 18) / rows : 1;  // short sequences have as many chunks as the longest: mostly empty workgroups
     if (c > 1024) c = 1024;
     if (c > most) c = most > 1 ? most : 1;
-    share = (tiles + c - 1) / c;
-    p.n_chunks = (int)((tiles + share - 1) / share);
-  } else {
-    share = tiles;
+    each = (tiles + c - 1) / c;
+    p.n_chunks = (int)((tiles + each - 1) / each);
   }
-  p.chunk = share * tile;
+  p.chunk = each * tile;
   return p;
 }
 

@@ -77,6 +77,8 @@ def test_gated_scan_refusals(L):
     # one long sequence needs the maps of its chunks, 16 tokens a step at a time nothing
     assert L.dc_gated_scan_workspace(100000, 64, 1, 100000) > 0 and L.dc_gated_scan_workspace(1600, 64, 100, 16) == 0
     refused(L, scan(L, n=100000, c=8, seqs=1, longest=100000), "workspace")
+    # a bound on the lengths is no more than the tokens, however large
+    assert L.dc_gated_scan_workspace(5000, 64, 2, 1 << 62) == L.dc_gated_scan_workspace(5000, 64, 2, 5000)
     assert L.dc_gated_scan_saved(0, 8) == 0 and L.dc_gated_scan_saved(1, 8) == 8 and L.dc_gated_scan_saved(65, 8) == 16
     assert L.dc_gated_scan_saved(1 << 33, 256) == 1 << 35
 
