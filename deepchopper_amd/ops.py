@@ -191,7 +191,7 @@ def summary_predict_dense(pred: torch.Tensor, labels: torch.Tensor, ignore_label
 
 
 # ------------------------------------------------------------------------------------------
-# sequence-layer and scoring operators
+# sequence-layer and scoring operators.  None of them is recorded by torch's autograd: the gradients are the *_backward functions'.
 # ------------------------------------------------------------------------------------------
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _TOKEN_TYPES = {torch.int8: 0, torch.uint8: 1, torch.int32: 2, torch.int64: 3}
@@ -258,7 +258,7 @@ def _rows(dev: int, name: str, t: torch.Tensor | None, shape: torch.Size | None 
 
 def _new_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """A dense tensor of `t`'s shape and device (`empty_like` takes half the time of `empty`)."""
-    return torch.empty_like(t) if t.dtype is dtype and t.is_contiguous() else torch.empty(t.shape, dtype=dtype, device=t.device)
+    return torch.empty_like(t) if t.dtype is dtype and t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
 
 
 def _address(t: torch.Tensor | None) -> int | None:
@@ -283,19 +283,19 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     classes))."""
     dev = _device_of("logits", logits)
     ptr, stride = _rows(dev, "logits", logits)
-    lead, n_classes, dtype, device = logits.shape[:-1], logits.shape[-1], logits.dtype, logits.device
+    lead, n_classes, dtype = logits.shape[:-1], logits.shape[-1], logits.dtype
     n = logits.numel() // n_classes if n_classes else 0
     tok, kind = _tokens(dev, tokens, lead)
-    logprob = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=device)
+    logprob = None if tokens is None else logits.new_empty(lead, dtype=torch.float32)
     entropy = None
     if want_entropy:
-        entropy = torch.empty_like(logprob) if logprob is not None else torch.empty(lead, dtype=torch.float32, device=device)
-    stats = torch.empty((n, 3), dtype=torch.float32, device=device) if save and n_classes >= STATS_FROM else None
-    ids = torch.empty((*lead, n_top), dtype=torch.int32, device=device) if n_top > 0 else None
-    top = torch.empty((*lead, n_top), dtype=torch.float32, device=device) if n_top > 0 else None
+        entropy = torch.empty_like(logprob) if logprob is not None else logits.new_empty(lead, dtype=torch.float32)
+    stats = logits.new_empty((n, 3), dtype=torch.float32) if save and n_classes >= STATS_FROM else None
+    ids = logits.new_empty((*lead, n_top), dtype=torch.int32) if n_top > 0 else None
+    top = logits.new_empty((*lead, n_top), dtype=torch.float32) if n_top > 0 else None
     L = _lib.lib()
     nb = L.dc_token_logprobs_workspace(n, n_classes, n_top) if n_classes >= STATS_FROM else 0
-    ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
+    ws = logits.new_empty(nb, dtype=torch.uint8) if nb else None
     with _on(dev):
         _lib.check(L.dc_token_logprobs(_stream_of(dev), ptr, _DTYPES[dtype], n, n_classes, stride, tok, kind, ignore_index, n_top, _address(logprob),
                                        _address(entropy), _address(stats), _address(ids), _address(top), _address(ws), nb))
@@ -363,12 +363,12 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, *, offsets: torch.Tensor | None
         out = _new_like(x, dtype) if begin is None else torch.zeros(shape, dtype=dtype, device=device)
     yp, ys = _rows(dev, "out", out, shape, dtype)
     if h_last is None:
-        h_last = torch.empty_like(h0) if h0 is not None else torch.empty((seqs, c), dtype=torch.float32, device=device)
+        h_last = torch.empty_like(h0) if h0 is not None else x.new_empty((seqs, c), dtype=torch.float32)
     hp = _like(dev, "h_last", h_last, (seqs, c), torch.float32)
     L = _lib.lib()
-    saved = torch.empty(L.dc_gated_scan_saved(n, c), dtype=torch.float32, device=device) if save else None
+    saved = x.new_empty(L.dc_gated_scan_saved(n, c), dtype=torch.float32) if save else None
     nb = L.dc_gated_scan_workspace(n, c, seqs, longest) if longest > 1 else 0
-    ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
+    ws = x.new_empty(nb, dtype=torch.uint8) if nb else None
     with _on(dev):
         _lib.check(L.dc_gated_scan(_stream_of(dev), _DTYPES[dtype], xp, xs, fp, fs, n, c, b, e, seqs, longest, int(reverse), h0p, yp, ys, int(zero_rest),
                                    hp, _address(saved), _address(ws), nb))
@@ -394,9 +394,9 @@ def gated_scan_backward(x: torch.Tensor, f: torch.Tensor, saved: torch.Tensor, g
         gx, gf = _new_like(x, dtype), _new_like(f, dtype)
     else:
         gx, gf = torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
-    gh = torch.empty((seqs, c), dtype=torch.float32, device=device)
+    gh = x.new_empty((seqs, c), dtype=torch.float32)
     nb = L.dc_gated_scan_workspace(n, c, seqs, longest)
-    ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
+    ws = x.new_empty(nb, dtype=torch.uint8) if nb else None
     with _on(dev):
         _lib.check(L.dc_gated_scan_backward(_stream_of(dev), _DTYPES[dtype], xp, xs, fp, fs, n, c, b, e, seqs, longest, int(reverse), h0p, sp, gp, gs,
                                             glp, gx.data_ptr(), c, gf.data_ptr(), c, int(offsets is not None), gh.data_ptr(), _address(ws), nb))
@@ -435,7 +435,7 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None = None, gat
     res_dtype = residual.dtype if residual is not None else act_dtype
     _need(act_dtype in _DTYPES, "block_norm: float32, float16 or bfloat16 required")
     _need(gate is None or y is not None, "gate: without a block's output")
-    shape, device = ref.shape, ref.device
+    shape = ref.shape
     w = shape[-1]
     yp, ys = _rows(dev, "y", y, shape)
     gp, gs = _rows(dev, "gate", gate, shape, act_dtype)
@@ -470,7 +470,7 @@ def block_norm_backward(y: torch.Tensor | None, residual: torch.Tensor | None = 
     res_dtype = residual.dtype if residual is not None else act_dtype
     _need(act_dtype in _DTYPES, "block_norm: float32, float16 or bfloat16 required")
     _need(gate is None or y is not None, "gate: without a block's output")
-    shape, device = ref.shape, ref.device
+    shape = ref.shape
     w = shape[-1]
     n = ref.numel() // w if w else 0
     yp, ys = _rows(dev, "y", y, shape)
@@ -485,7 +485,7 @@ def block_norm_backward(y: torch.Tensor | None, residual: torch.Tensor | None = 
     _like(dev, "pre_bias", pre_bias, one, torch.float32)
 
     normed = post and y is not None
-    sums = torch.empty((5, w), dtype=torch.float32, device=device).unbind()
+    sums = ref.new_empty((5, w), dtype=torch.float32).unbind()
     wanted = (y is not None and scale is not None, normed and post_weight is not None, normed and post_bias is not None, pre_weight is not None,
               pre_bias is not None)
     vectors = [t if want else None for t, want in zip(sums, wanted)]
@@ -494,7 +494,7 @@ def block_norm_backward(y: torch.Tensor | None, residual: torch.Tensor | None = 
     gr = None if residual is None else _new_like(residual, res_dtype)
     L = _lib.lib()
     nb = L.dc_block_norm_workspace(n, w, _DTYPES[res_dtype])
-    ws = torch.empty(nb, dtype=torch.uint8, device=device) if nb else None
+    ws = ref.new_empty(nb, dtype=torch.uint8) if nb else None
     with _on(dev):
         _lib.check(L.dc_block_norm_backward(
             _stream_of(dev), _DTYPES[act_dtype], _DTYPES[res_dtype], n, w, k, eps, yp, ys, gp, gs, act, rp, rs, sc, int(post), pw, pb, qw, grp, grs,
