@@ -26,7 +26,6 @@ constexpr int kTile = 64;      // tokens between two states of d_saved
 constexpr int kThreads = 512;  // a workgroup
 constexpr int kSteps = 8;      // consecutive tokens of one group of lanes: their inputs live in registers
 constexpr int kShort = 16;     // sequences up to here: a thread per channel, token after token
-constexpr int kZeroBlocks = 32;
 
 struct ScanArgs {
   const int64_t* begin;  // or null: dense sequences of max_len tokens
@@ -36,7 +35,7 @@ struct ScanArgs {
   int32_t lane_bits;  // log2 of the lanes along the channels
   int32_t n_chunks;   // chunks of a sequence ...
   int64_t chunk;      // ... of so many tokens each (a multiple of the workgroup's tile)
-  int32_t n_blocks;   // workgroups of the recurrence; those behind them write the zeros of zero_rest
+  int32_t n_blocks;   // workgroups of the recurrence; those behind them are fill_rest's
   int32_t whole;      // every lane has channels and all strides are at most 2^20: tiles inside a sequence need no checks
 };
 
@@ -46,6 +45,9 @@ __device__ __forceinline__ int64_t scalar(int64_t v) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
+// whether [b, e) is a sequence of this call; one that is not is refused
+__device__ __forceinline__ bool fits(const ScanArgs& a, int64_t b, int64_t e) { return b >= 0 && e >= b && e <= a.n_tokens && e - b <= a.max_len; }
+
 // A sequence in the order of the recurrence: its token j is row base + dir * j.
 struct Seq {
   int64_t base, len;
@@ -53,7 +55,7 @@ struct Seq {
   bool ok;
   __device__ __forceinline__ Seq(const ScanArgs& a, int s) {
     const int64_t b = scalar(a.begin ? a.begin[s] : s * a.max_len), e = scalar(a.end ? a.end[s] : b + a.max_len);
-    ok = b >= 0 && e >= b && e <= a.n_tokens && e - b <= a.max_len;
+    ok = fits(a, b, e);
     len = ok ? e - b : 0;
     base = a.reverse ? e - 1 : b;
     dir = a.reverse ? -1 : 1;
@@ -97,24 +99,46 @@ __device__ __forceinline__ Span then(const Span& a, const Span& b) {  // a, then
   return {a.A * b.A, __builtin_fmaf(b.G, 1.0f - a.G, a.G), apply(b.A, b.G, b.H, a.H)};
 }
 
-// the rows in front of the first and behind the last sequence, to zero
+__device__ __forceinline__ int64_t inside(const ScanArgs& a, int64_t t) { return t < 0 ? 0 : t > a.n_tokens ? a.n_tokens : t; }
+
+// zero_rest, by the workgroups behind the recurrence's: the rows in front of the first and behind the last sequence to zero, and those of a
+// refused sequence to NaN.  Every lane looks at a sequence; the wavefront writes the rows of those that are refused, one after the other.
 template <typename T>
-__device__ void zero_rest(const ScanArgs& a, int block, T* y, int64_t ldy, T* y2, int64_t ldy2) {
+__device__ void fill_rest(const ScanArgs& a, T* y, int64_t ldy, T* y2, int64_t ldy2) {
+  const int block = blockIdx.x - a.n_blocks, n_blocks = gridDim.x - a.n_blocks;
   int64_t b = a.n_tokens, e = a.n_tokens;
   if (a.n_seqs > 0) {
-    b = a.begin ? a.begin[0] : 0;
-    e = a.end ? a.end[a.n_seqs - 1] : a.n_seqs * a.max_len;
-    b = b < 0 ? 0 : b > a.n_tokens ? a.n_tokens : b;
-    e = e < b ? b : e > a.n_tokens ? a.n_tokens : e;
+    b = inside(a, a.begin ? a.begin[0] : 0);
+    e = inside(a, a.end ? a.end[a.n_seqs - 1] : a.n_seqs * a.max_len);
+    e = e < b ? b : e;
   }
-  for (int64_t i = block; i < b + a.n_tokens - e; i += kZeroBlocks) {
+  for (int64_t i = block; i < b + a.n_tokens - e; i += n_blocks) {
     const int64_t t = i < b ? i : i - b + e;
     for (int c = threadIdx.x; c < a.n_channels; c += blockDim.x) {
       y[t * ldy + c] = (T)0.0f;
       if (y2) y2[t * ldy2 + c] = (T)0.0f;
     }
   }
+  if (!a.begin) return;  // (dense sequences are checked on the host)
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  for (int64_t first = (int64_t)(block * waves + (int)(threadIdx.x >> 6)) * 64; first < a.n_seqs; first += (int64_t)n_blocks * waves * 64) {
+    const int64_t s = first + lane;
+    bool refused = false;
+    if (s < a.n_seqs) b = a.begin[s], e = a.end[s], refused = !fits(a, b, e);
+    for (uint64_t left = __ballot(refused); left; left &= left - 1) {
+      const int64_t r = first + __builtin_ctzll(left), rb = inside(a, a.begin[r]), re = inside(a, a.end[r]);
+      for (int64_t t = rb; t < re; ++t) {
+        for (int c = lane; c < a.n_channels; c += 64) {
+          y[t * ldy + c] = (T)__builtin_nanf("");
+          if (y2) y2[t * ldy2 + c] = (T)__builtin_nanf("");
+        }
+      }
+    }
+  }
 }
+
+// workgroups of fill_rest (as small as 64 threads): a wavefront looks at no more than a few times 64 sequences
+int rest_blocks(int64_t n_tokens, int32_t n_seqs, int32_t zero_rest) { return zero_rest && n_tokens > 0 ? 32 + n_seqs / 256 : 0; }
 
 // Of an odd number of channels the last lane takes the last two and writes only the second: the first is its neighbour's.
 template <int V, typename T>
@@ -129,7 +153,7 @@ constexpr int kWalkThreads = 64;
 template <typename T, int V>
 __global__ __launch_bounds__(kWalkThreads) void scan_walk_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f, int64_t ldf,
                                                                  const float* h0, T* __restrict__ y, int64_t ldy, float* h_last) {
-  if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, y, ldy, nullptr, 0);
+  if ((int)blockIdx.x >= a.n_blocks) return fill_rest<T>(a, y, ldy, nullptr, 0);
   const int per_seq = (a.n_channels + kWalkThreads * V - 1) / (kWalkThreads * V);
   const int s = blockIdx.x / per_seq;
   int c = (blockIdx.x % per_seq * kWalkThreads + threadIdx.x) * V;
@@ -167,7 +191,7 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_backward_kernel(ScanAr
                                                                           const float* __restrict__ h0, const T* __restrict__ gy, int64_t ldgy,
                                                                           const float* g_last, T* __restrict__ gx, int64_t ldgx, T* __restrict__ gf,
                                                                           int64_t ldgf, float* g_h0) {
-  if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, gx, ldgx, gf, ldgf);
+  if ((int)blockIdx.x >= a.n_blocks) return fill_rest<T>(a, gx, ldgx, gf, ldgf);
   __shared__ float above[kShort][kWalkThreads * V];  // h_(t-1) - x_t
   const int per_seq = (a.n_channels + kWalkThreads * V - 1) / (kWalkThreads * V);
   const int s = blockIdx.x / per_seq;
@@ -392,7 +416,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, cons
                                                                 const float* h0, T* __restrict__ y, int64_t ldy, float* h_last,
                                                                 float* __restrict__ saved, const float* __restrict__ maps) {
   __shared__ float lds[2][3][kThreads * V], ends[2][64 * V];
-  if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, y, ldy, nullptr, 0);
+  if ((int)blockIdx.x >= a.n_blocks) return fill_rest<T>(a, y, ldy, nullptr, 0);
   const Place<V> at(a);
   const Seq q(a, at.s);
   const int lanes_v = V << a.lane_bits, tile = at.n_groups * kSteps;
@@ -493,7 +517,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_backward_kernel(ScanArg
                                                                          T* __restrict__ gx, int64_t ldgx, T* __restrict__ gf, int64_t ldgf, float* g_h0,
                                                                          const float* __restrict__ maps) {
   __shared__ float lds[2][4][kThreads * V], ends[2][64 * V];
-  if ((int)blockIdx.x >= a.n_blocks) return zero_rest<T>(a, blockIdx.x - a.n_blocks, gx, ldgx, gf, ldgf);
+  if ((int)blockIdx.x >= a.n_blocks) return fill_rest<T>(a, gx, ldgx, gf, ldgf);
   const Place<V> at(a);
   const Seq q(a, at.s);
   const int lanes_v = V << a.lane_bits, tile = at.n_groups * kSteps;
@@ -728,26 +752,26 @@ extern "C" int dc_gated_scan(void* stream, int32_t dtype, const void* d_x, int64
   const int v = channels_per_lane(dtype, n_channels);
   const Plan p = scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
   ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0, whole_tiles(p, n_channels, {x_stride, f_stride, y_stride})};
-  const int zeros = zero_rest && n_tokens > 0 ? kZeroBlocks : 0;
+  const int rest = rest_blocks(n_tokens, n_seqs, zero_rest);
   return with_lanes(dtype, v, [&](auto t, auto lanes) {
     using T = decltype(t);
     constexpr int V = decltype(lanes)::value;
     const T *x = (const T*)d_x, *f = (const T*)d_f;
     if (max_len <= kShort) {
       a.n_blocks = n_seqs * ((n_channels + kWalkThreads * V - 1) / (kWalkThreads * V));
-      if (a.n_blocks + zeros == 0) return DC_OK;
-      scan_walk_kernel<T, V><<<dim3(a.n_blocks + zeros), dim3(kWalkThreads), 0, as_stream(stream)>>>(a, x, x_stride, f, f_stride, d_h0, (T*)d_y, y_stride, d_h_last);
+      if (a.n_blocks + rest == 0) return DC_OK;
+      scan_walk_kernel<T, V><<<dim3(a.n_blocks + rest), dim3(kWalkThreads), 0, as_stream(stream)>>>(a, x, x_stride, f, f_stride, d_h0, (T*)d_y, y_stride, d_h_last);
       DC_LAUNCH_CHECK();
       return DC_OK;
     }
     a.n_blocks = n_seqs * p.per_row * p.n_chunks;
-    if (a.n_blocks + zeros == 0) return DC_OK;
+    if (a.n_blocks + rest == 0) return DC_OK;
     float* maps = p.n_chunks > 1 ? (float*)d_workspace : nullptr;
     if (maps) {
       scan_map_kernel<T, V, false><<<dim3(a.n_blocks), dim3(kThreads), 0, as_stream(stream)>>>(a, f, f_stride, x, x_stride, d_h0, maps);
       DC_LAUNCH_CHECK();
     }
-    scan_tile_kernel<T, V><<<dim3(a.n_blocks + zeros), dim3(kThreads), 0, as_stream(stream)>>>(a, x, x_stride, f, f_stride, d_h0, (T*)d_y, y_stride, d_h_last,
+    scan_tile_kernel<T, V><<<dim3(a.n_blocks + rest), dim3(kThreads), 0, as_stream(stream)>>>(a, x, x_stride, f, f_stride, d_h0, (T*)d_y, y_stride, d_h_last,
                                                                                                d_saved, maps);
     DC_LAUNCH_CHECK();
     return DC_OK;
@@ -768,7 +792,7 @@ extern "C" int dc_gated_scan_backward(void* stream, int32_t dtype, const void* d
   const int v = channels_per_lane(dtype, n_channels);
   const Plan p = scan_plan(n_tokens, n_channels, n_seqs, max_len, v);
   ScanArgs a{d_begin, d_end, n_tokens, max_len, n_seqs, n_channels, reverse, p.lane_bits, p.n_chunks, p.chunk, 0, whole_tiles(p, n_channels, {x_stride, f_stride, grad_y_stride, grad_x_stride, grad_f_stride})};
-  const int zeros = zero_rest && n_tokens > 0 ? kZeroBlocks : 0;
+  const int rest = rest_blocks(n_tokens, n_seqs, zero_rest);
   return with_lanes(dtype, v, [&](auto t, auto lanes) {
     using T = decltype(t);
     constexpr int V = decltype(lanes)::value;
@@ -776,20 +800,20 @@ extern "C" int dc_gated_scan_backward(void* stream, int32_t dtype, const void* d
     T *gx = (T*)d_grad_x, *gf = (T*)d_grad_f;
     if (max_len <= kShort) {
       a.n_blocks = n_seqs * ((n_channels + kWalkThreads * V - 1) / (kWalkThreads * V));
-      if (a.n_blocks + zeros == 0) return DC_OK;
-      scan_walk_backward_kernel<T, V><<<dim3(a.n_blocks + zeros), dim3(kWalkThreads), 0, as_stream(stream)>>>(
+      if (a.n_blocks + rest == 0) return DC_OK;
+      scan_walk_backward_kernel<T, V><<<dim3(a.n_blocks + rest), dim3(kWalkThreads), 0, as_stream(stream)>>>(
           a, x, x_stride, f, f_stride, d_h0, gy, grad_y_stride, d_grad_h_last, gx, grad_x_stride, gf, grad_f_stride, d_grad_h0);
       DC_LAUNCH_CHECK();
       return DC_OK;
     }
     a.n_blocks = n_seqs * p.per_row * p.n_chunks;
-    if (a.n_blocks + zeros == 0) return DC_OK;
+    if (a.n_blocks + rest == 0) return DC_OK;
     float* maps = p.n_chunks > 1 ? (float*)d_workspace : nullptr;
     if (maps) {
       scan_map_kernel<T, V, true><<<dim3(a.n_blocks), dim3(kThreads), 0, as_stream(stream)>>>(a, f, f_stride, gy, grad_y_stride, d_grad_h_last, maps);
       DC_LAUNCH_CHECK();
     }
-    scan_tile_backward_kernel<T, V><<<dim3(a.n_blocks + zeros), dim3(kThreads), 0, as_stream(stream)>>>(
+    scan_tile_backward_kernel<T, V><<<dim3(a.n_blocks + rest), dim3(kThreads), 0, as_stream(stream)>>>(
         a, x, x_stride, f, f_stride, d_h0, d_saved, gy, grad_y_stride, d_grad_h_last, gx, grad_x_stride, gf, grad_f_stride, d_grad_h0, maps);
     DC_LAUNCH_CHECK();
     return DC_OK;

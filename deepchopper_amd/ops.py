@@ -351,7 +351,9 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, *, offsets: torch.Tensor | None
     x, f [n_seqs, length, n_channels] dense, or [n_tokens, n_channels] with the sequences at `offsets` int64[n_seqs + 1], or at
     `begin` / `end` int64[n_seqs] (left-padded rows: first column and end of each).  `h0` f32[n_seqs, n_channels] state to start from; `reverse`: from
     the sequences' ends.  `h_last` may be given (`h0` itself: a state kept in place while bases stream in); `out` keeps what stands in
-    tokens of no sequence, which are zero otherwise.  Returns dict(y, h_last, saved: for `gated_scan_backward`, with `save`)."""
+    tokens of no sequence, which are zero otherwise.  `max_len`: no sequence is longer (found on the host, with a wait, where it is not
+    given).  A sequence that is, or that leaves the tokens, is refused: NaN in its row of h_last and, with `offsets`, in its rows of y; with
+    `begin` / `end` or a given `out` those stay as tokens of no sequence.  Returns dict(y, h_last, saved: for `gated_scan_backward`, with `save`)."""
     dev = _device_of("x", x)
     xp, xs = _rows(dev, "x", x)
     shape, dtype, device = x.shape, x.dtype, x.device
@@ -379,7 +381,7 @@ def gated_scan_backward(x: torch.Tensor, f: torch.Tensor, saved: torch.Tensor, g
                         h0: torch.Tensor | None = None, offsets: torch.Tensor | None = None, begin: torch.Tensor | None = None,
                         end: torch.Tensor | None = None, max_len: int | None = None, reverse: bool = False) -> dict:
     """Gradients of `gated_scan` for `grad_y` (and `grad_h_last`): dict(grad_x, grad_f, grad_h0 f32[n_seqs, n_channels]).  The other
-    arguments as in the forward call, `saved` as it returned it; tokens of no sequence get zeros."""
+    arguments as in the forward call, `saved` as it returned it; tokens of no sequence get zeros, refused sequences what they get in y."""
     dev = _device_of("x", x)
     xp, xs = _rows(dev, "x", x)
     shape, dtype, device = x.shape, x.dtype, x.device

@@ -456,11 +456,13 @@ int dc_token_logprobs_backward(void* stream, const void* d_logits, int32_t dtype
  *  max_len    : no sequence is longer (host value: it shapes the launch)
  *  d_h0       : float[n_seqs, n_channels] state before the first token, or NULL (zeros)
  *  d_y        : [n_tokens, n_channels], not overlapping the inputs; tokens of no sequence are left untouched, or with
- *               zero_rest != 0 those in front of begin[0] and from end[n_seqs - 1] on (all, where there is no sequence) set to 0
+ *               zero_rest != 0 (packed sequences: begin ascending, end[s] = begin[s + 1]) those in front of begin[0] and from
+ *               end[n_seqs - 1] on (all, where there is no sequence) set to 0 and those of a refused sequence to NaN
  *  d_h_last   : float[n_seqs, n_channels] state after the last token, or NULL; it may be d_h0 (a state kept in place)
  *  d_saved    : dc_gated_scan_saved(...) floats for the backward pass, or NULL
  *  A sequence with begin < 0, end < begin, end > n_tokens or more than max_len tokens is refused on the device: its d_h_last
- *  row (backward: d_grad_h0 row) is NaN and nothing else of it is written. */
+ *  row (backward: d_grad_h0 row) is NaN, and so are with zero_rest != 0 its rows of d_y (d_grad_x, d_grad_f) inside the
+ *  tokens; nothing else of it is written. */
 int dc_gated_scan(void* stream, int32_t dtype, const void* d_x, int64_t x_stride, const void* d_f, int64_t f_stride,
                   int64_t n_tokens, int32_t n_channels, const int64_t* d_begin, const int64_t* d_end, int32_t n_seqs,
                   int64_t max_len, int32_t reverse, const float* d_h0, void* d_y, int64_t y_stride, int32_t zero_rest,
