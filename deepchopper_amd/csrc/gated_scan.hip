@@ -6,6 +6,10 @@
 // so a gate that keeps 99.99 % for thousands of tokens loses no more than one that forgets at once (with a rounded, a h would
 // drift by 2^-25 a step).  A span of steps is the map h -> H + A h; it carries both A and G = 1 - A and is applied with the
 // smaller of them, for the same reason.  Weights below 2^-126 are 0.
+// x - h can be beyond fp32 where a h + (1 - a) x is not, and is NaN for an infinite state.  A state (or gradient) that is not finite stays
+// so to the end of a group's 8 tokens, a span's passes to the groups behind: the last one of every 8 tells, and at the end a thread walks
+// such a channel once more, token after token, with the sure_ forms (100 001 x 256 fp32 with gradients: 229 us without that, 233 us with;
+// 1 024 sequences of 500 - 1 500 x 256 bf16: 341 us both).
 //
 // Form.  HBM-bound: 3 elements of traffic per element forward, 5 backward, about 35 and 50 vector operations.  Lanes run along the
 // channels (a row of 64 lanes is 256 contiguous bytes), time is divided: a workgroup's 8 wavefronts take 8 consecutive tokens each of
@@ -70,6 +74,42 @@ __device__ __forceinline__ float step(float h, float x, float ps) { return __bui
 // a * v
 __device__ __forceinline__ float decay(float v, float ps) { return keeps(ps) ? __builtin_fmaf(-ps, v, v) : -ps * v; }
 
+__device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) < INFINITY; }
+template <int V>
+__device__ __forceinline__ bool all_finite(const float (&h)[V]) {
+  bool ok = true;
+#pragma unroll
+  for (int v = 0; v < V; ++v) ok = ok && finite(h[v]);
+  return ok;
+}
+constexpr float kLeast = 1.17549435e-38f, kMost = 3.40282347e+38f;  // normal fp32 numbers
+
+// The factor a of a state or gradient v: an infinite one stays infinite however small a is (where a is 0 in fp32 too).
+__device__ __forceinline__ float weight_of(float a, float v) { return __builtin_fabsf(v) == INFINITY ? __builtin_fmaxf(a, kLeast) : a; }
+
+// step and decay; where those leave fp32, from the two products (a step between finite operands does not leave them)
+__device__ __forceinline__ float sure_step(float h, float x, float ps) {
+  float r = step(h, x, ps);
+  if (__builtin_expect(!finite(r), 0)) {
+    const float p = __builtin_fabsf(ps), q = 1.0f - p;
+    r = __builtin_fmaf(weight_of(keeps(ps) ? q : p, h), h, (keeps(ps) ? p : q) * x);
+    if (finite(h) && finite(x)) r = __builtin_amdgcn_fmed3f(r, h, x);
+  }
+  return r;
+}
+__device__ __forceinline__ float sure_decay(float v, float ps) {
+  const float r = decay(v, ps), p = __builtin_fabsf(ps);
+  return finite(r) ? r : weight_of(keeps(ps) ? 1.0f - p : p, v) * v;
+}
+
+// One token's gradients from half of h_(t-1) - x_t (the whole may be beyond fp32) and g_t; g_t becomes a_t g_t.
+__device__ __forceinline__ void sure_back(float& g, float ps, float half, float& dx, float& df) {
+  const float p = __builtin_fabsf(ps), part = p * g, rest = finite(g) ? __builtin_fmaf(-p, g, g) : (1.0f - p) * g;
+  dx = keeps(ps) ? part : rest;
+  df = p * rest * half * 2.0f;
+  g = sure_decay(g, ps);
+}
+
 // Comparisons made of ps so far are not kept (in scalar registers that spill) but made again.
 template <int V>
 __device__ __forceinline__ void forget(float (&ps)[kSteps][V]) {
@@ -97,6 +137,14 @@ __device__ __forceinline__ void extend(float& A, float& G, float ps) {  // by on
 }
 __device__ __forceinline__ Span then(const Span& a, const Span& b) {  // a, then b
   return {a.A * b.A, __builtin_fmaf(b.G, 1.0f - a.G, a.G), apply(b.A, b.G, b.H, a.H)};
+}
+// apply where that leaves fp32: a state, between finite H and h, by rounding alone; a gradient (BACK) on the way
+template <bool BACK>
+__device__ __forceinline__ float sure_apply(float A, float G, float H, float h) {
+  const float r = apply(A, G, H, h);
+  if (finite(r)) return r;
+  if (!BACK && finite(h) && finite(H)) return __builtin_amdgcn_fmed3f(r, -kMost, kMost);
+  return __builtin_fmaf(weight_of(A, h), h, H);
 }
 
 __device__ __forceinline__ int64_t inside(const ScanArgs& a, int64_t t) { return t < 0 ? 0 : t > a.n_tokens ? a.n_tokens : t; }
@@ -174,7 +222,7 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_kernel(ScanArgs a, con
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float ps = signed_gate(fv[v]);
-      h[v] = step(h[v], seen(xv[v], ps), ps);
+      h[v] = sure_step(h[v], seen(xv[v], ps), ps);
     }
     store_channels<V>(y + t * ldy + c, h, second);
   }
@@ -192,7 +240,7 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_backward_kernel(ScanAr
                                                                           const float* g_last, T* __restrict__ gx, int64_t ldgx, T* __restrict__ gf,
                                                                           int64_t ldgf, float* g_h0) {
   if ((int)blockIdx.x >= a.n_blocks) return fill_rest<T>(a, gx, ldgx, gf, ldgf);
-  __shared__ float above[kShort][kWalkThreads * V];  // h_(t-1) - x_t
+  __shared__ float half[kShort][kWalkThreads * V];  // of h_(t-1) - x_t
   const int per_seq = (a.n_channels + kWalkThreads * V - 1) / (kWalkThreads * V);
   const int s = blockIdx.x / per_seq;
   int c = (blockIdx.x % per_seq * kWalkThreads + threadIdx.x) * V;
@@ -214,8 +262,8 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_backward_kernel(ScanAr
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float ps = signed_gate(fv[v]), xs = seen(xv[v], ps);
-      above[j][threadIdx.x * V + v] = h[v] - xs;
-      h[v] = step(h[v], xs, ps);
+      half[j][threadIdx.x * V + v] = __builtin_fmaf(-0.5f, xs, 0.5f * h[v]);
+      h[v] = sure_step(h[v], xs, ps);
     }
   }
 #pragma unroll 4
@@ -226,11 +274,8 @@ __global__ __launch_bounds__(kWalkThreads) void scan_walk_backward_kernel(ScanAr
     load_vec<V>(gy + t * ldgy + c, yv);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float ps = signed_gate(fv[v]), p = __builtin_fabsf(ps);
-      const float total = g[v] + yv[v], part = p * total, rest = __builtin_fmaf(-p, total, total);
-      ox[v] = keeps(ps) ? part : rest;
-      g[v] = keeps(ps) ? rest : part;
-      of[v] = p * rest * above[j][threadIdx.x * V + v];
+      g[v] += yv[v];
+      sure_back(g[v], signed_gate(fv[v]), half[j][threadIdx.x * V + v], ox[v], of[v]);
     }
     store_channels<V>(gx + t * ldgx + c, ox, second);
     store_channels<V>(gf + t * ldgf + c, of, second);
@@ -357,6 +402,14 @@ __global__ __launch_bounds__(kThreads) void scan_map_kernel(ScanArgs a, const T*
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
+    if (__builtin_expect(!finite(m[v].H), 0)) {
+      m[v].H = 0.0f;
+      for (int64_t k = p0; k < p1; ++k) {
+        const int64_t t = q.row(BACK ? p1 - 1 - (k - p0) : k);
+        const float ps = signed_gate((float)f[t * ldf + at.channel + v]), xv = (float)x[t * ldx + at.channel + v];
+        m[v].H = BACK ? sure_decay(m[v].H + xv, ps) : sure_step(m[v].H, seen(xv, ps), ps);
+      }
+    }
     const int i = at.at(at.group, lanes_v) + v;
     lds[0][i] = m[v].A, lds[1][i] = m[v].G, lds[2][i] = m[v].H;
   }
@@ -366,7 +419,9 @@ __global__ __launch_bounds__(kThreads) void scan_map_kernel(ScanArgs a, const T*
     Span all = identity_span();
     for (int k = 0; k < at.n_groups; ++k) {
       const int i = at.at(BACK ? at.n_groups - 1 - k : k, lanes_v) + v;
+      const float H = sure_apply<BACK>(lds[0][i], lds[1][i], lds[2][i], all.H);
       all = then(all, Span{lds[0][i], lds[1][i], lds[2][i]});
+      all.H = H;
     }
     maps[map_at(a, at.s, at.chunk, 0, at.channel + v)] = all.A;
     maps[map_at(a, at.s, at.chunk, 1, at.channel + v)] = all.G;
@@ -411,11 +466,139 @@ __device__ void compose_chunks(const ScanArgs& a, const Place<V>& at, const floa
   __syncthreads();
 }
 
+// What a chunk starts from, by one thread with the sure forms: `start` (h0 or the gradient of h_last, or null) where there are no maps.
+template <bool BACK, int V>
+__device__ __forceinline__ void sure_start(const ScanArgs& a, const Place<V>& at, const float* maps, const float* start, int from, int dir, int n, float (&h)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    h[v] = maps ? maps[start_at(a, at.s, at.channel + v)] : start ? start[(int64_t)at.s * a.n_channels + at.channel + v] : 0.0f;
+    for (int k = 0; maps && k < n; ++k) {
+      const int64_t i = map_at(a, at.s, from + dir * k, 0, at.channel + v);
+      h[v] = sure_apply<BACK>(maps[i], maps[i + a.n_channels], maps[i + 2 * (int64_t)a.n_channels], h[v]);
+    }
+  }
+}
+
+// A kernel's own arguments, loaded (again) where this stands: what only the second walk looks at is not kept in (spilling) scalar registers
+// through the loops in front of it (3 300 sequences of 29 - 38 x 43 fp32: 24.2 us kept, 22.9 us loaded).  Arguments lie one after the
+// other, each at its alignment; these structs name them in the kernels' order.
+template <typename Args>
+__device__ __forceinline__ const Args& own_arguments() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Args*)p;
+}
+
+// scan_tile_kernel's
+template <typename T>
+struct TileArgs {
+  ScanArgs a;
+  const T* x;
+  int64_t ldx;
+  const T* f;
+  int64_t ldf;
+  const float* h0;
+  T* y;
+  int64_t ldy;
+  float *h_last, *saved;
+  const float* maps;
+};
+// scan_tile_backward_kernel's
+template <typename T>
+struct TileBackArgs {
+  ScanArgs a;
+  const T* x;
+  int64_t ldx;
+  const T* f;
+  int64_t ldf;
+  const float *h0, *saved;
+  const T* gy;
+  int64_t ldgy;
+  const float* g_last;
+  T* gx;
+  int64_t ldgx;
+  T* gf;
+  int64_t ldgf;
+  float* g_h0;
+  const float* maps;
+};
+
+// A chunk's tokens for a thread's channels, one after the other, with the sure forms: the states written again; h: the last one.
+template <typename T, int V>
+__device__ __forceinline__ void sure_walk(const TileArgs<T>& k, float (&h)[V]) {
+  const Place<V> at(k.a);
+  const Seq q(k.a, at.s);
+  const int64_t j0 = at.chunk * k.a.chunk, j1 = j0 + k.a.chunk < q.len ? j0 + k.a.chunk : q.len;
+  sure_start<false, V>(k.a, at, k.maps, k.h0, 0, 1, at.chunk, h);
+#pragma unroll 1
+  for (int64_t j = j0; j < j1; ++j) {
+    const int64_t t = q.row(j);
+    if (k.saved && j % kTile == 0 && j > 0) store_channels<V>(k.saved + (t / kTile * k.a.n_channels + at.channel), h, at.second);
+    float xv[V], fv[V];
+    load_vec<V>(k.x + t * k.ldx + at.channel, xv);
+    load_vec<V>(k.f + t * k.ldf + at.channel, fv);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float ps = signed_gate(fv[v]);
+      h[v] = sure_step(h[v], seen(xv[v], ps), ps);
+    }
+    store_channels<V>(k.y + t * k.ldy + at.channel, h, at.second);
+  }
+}
+
+// ... and their gradients, from the last token back, kTile tokens from each state of `saved`; c: what comes out of the first one.  `lds`:
+// half of h_(t-1) - x_t for kTile tokens.
+template <typename T, int V>
+__device__ __forceinline__ void sure_walk_back(const TileBackArgs<T>& k, float* lds, float (&c)[V]) {
+  const Place<V> at(k.a);
+  const Seq q(k.a, at.s);
+  const int64_t j0 = at.chunk * k.a.chunk, j1 = j0 + k.a.chunk < q.len ? j0 + k.a.chunk : q.len;
+  const int last = q.len > 0 ? (int)((q.len - 1) / k.a.chunk) : 0, lanes_v = V << k.a.lane_bits;
+  float* half = lds + at.slot;
+  sure_start<true, V>(k.a, at, k.maps, k.g_last, last, -1, last - at.chunk, c);
+#pragma unroll 1
+  for (int64_t jt = j0 + (j1 - j0 - 1) / kTile * kTile; j1 > j0 && jt >= j0; jt -= kTile) {
+    const int n = j1 - jt < kTile ? (int)(j1 - jt) : kTile;
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      h[v] = jt > 0 ? k.saved[q.row(jt) / kTile * k.a.n_channels + at.channel + v] : k.h0 ? k.h0[(int64_t)at.s * k.a.n_channels + at.channel + v] : 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const int64_t t = q.row(jt + i);
+      float xv[V], fv[V];
+      load_vec<V>(k.x + t * k.ldx + at.channel, xv);
+      load_vec<V>(k.f + t * k.ldf + at.channel, fv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float ps = signed_gate(fv[v]), xs = seen(xv[v], ps);
+        half[i * lanes_v + v] = __builtin_fmaf(-0.5f, xs, 0.5f * h[v]);
+        h[v] = sure_step(h[v], xs, ps);
+      }
+    }
+#pragma unroll 1
+    for (int i = n - 1; i >= 0; --i) {
+      const int64_t t = q.row(jt + i);
+      float fv[V], yv[V], dx[V], df[V];
+      load_vec<V>(k.f + t * k.ldf + at.channel, fv);
+      load_vec<V>(k.gy + t * k.ldgy + at.channel, yv);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        c[v] += yv[v];
+        sure_back(c[v], signed_gate(fv[v]), half[i * lanes_v + v], dx[v], df[v]);
+      }
+      store_channels<V>(k.gx + t * k.ldgx + at.channel, dx, at.second);
+      store_channels<V>(k.gf + t * k.ldgf + at.channel, df, at.second);
+    }
+  }
+}
+
 template <typename T, int V>
 __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, const T* __restrict__ x, int64_t ldx, const T* __restrict__ f, int64_t ldf,
                                                                 const float* h0, T* __restrict__ y, int64_t ldy, float* h_last,
                                                                 float* __restrict__ saved, const float* __restrict__ maps) {
   __shared__ float lds[2][3][kThreads * V], ends[2][64 * V];
+  __shared__ int lost[64];  // a lane's states left the finite numbers somewhere
   if ((int)blockIdx.x >= a.n_blocks) return fill_rest<T>(a, y, ldy, nullptr, 0);
   const Place<V> at(a);
   const Seq q(a, at.s);
@@ -423,6 +606,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, cons
   const int64_t sc = (int64_t)at.s * a.n_channels + at.channel;
   const int64_t j0 = at.chunk * a.chunk, j1 = j0 + a.chunk < q.len ? j0 + a.chunk : q.len;
   if (j0 >= q.len && at.chunk > 0) return;
+  if (threadIdx.x < 64) lost[threadIdx.x] = 0;  // (set behind the last tile; without a tile there is nothing to walk again)
   float carry[V];
   if (maps) {
     compose_chunks<V>(a, at, maps, 0, 1, at.chunk, lds[0], carry);
@@ -430,6 +614,9 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, cons
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = h0 && at.active ? h0[sc + v] : 0.0f;
   }
+  float trace = 0.0f;  // NaN once something is not finite
+#pragma unroll
+  for (int v = 0; v < V; ++v) trace = __builtin_fmaf(carry[v], 0.0f, trace);
   const TileRows<T, V> tx(at, q, ldx), tf(at, q, ldf), ty(at, q, ldy);
   const int64_t sx = q.dir * ldx, sf = q.dir * ldf, sy = q.dir * ldy;
   const bool last_group = at.group == at.n_groups - 1;
@@ -491,6 +678,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, cons
         else if (i < n) store_channels<V>(out + i * sy, h, at.second);
       }
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v) trace = __builtin_fmaf(h[v], 0.0f, trace);
     if (last_group) {  // the state behind the tile, for the next one
 #pragma unroll
       for (int v = 0; v < V; ++v) ends[turn][at.slot + v] = carry[v] = h[v];
@@ -501,6 +690,14 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, cons
   if (a.whole)
     for (; jt + tile <= j1; jt += tile) one_tile(std::true_type{}, jt);
   for (; jt < j1; jt += tile) one_tile(std::false_type{}, jt);
+  if (__builtin_expect(trace != 0.0f, 0)) lost[at.slot / V] = 1;
+  __syncthreads();  // (what the other groups have stored is written again behind them)
+  if (__builtin_expect(last_group && at.active && lost[at.slot / V], 0)) {
+    float h[V];
+    sure_walk<T, V>(own_arguments<TileArgs<T>>(), h);
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = h[v];
+  }
   if (h_last && last_group && at.active && j1 == q.len) {
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = q.ok ? carry[v] : __builtin_nanf("");
@@ -517,6 +714,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_backward_kernel(ScanArg
                                                                          T* __restrict__ gx, int64_t ldgx, T* __restrict__ gf, int64_t ldgf, float* g_h0,
                                                                          const float* __restrict__ maps) {
   __shared__ float lds[2][4][kThreads * V], ends[2][64 * V];
+  __shared__ int lost[64];  // a lane's states or gradients left the finite numbers somewhere
   if ((int)blockIdx.x >= a.n_blocks) return fill_rest<T>(a, gx, ldgx, gf, ldgf);
   const Place<V> at(a);
   const Seq q(a, at.s);
@@ -524,6 +722,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_backward_kernel(ScanArg
   const int64_t sc = (int64_t)at.s * a.n_channels + at.channel;
   const int64_t j0 = at.chunk * a.chunk, j1 = j0 + a.chunk < q.len ? j0 + a.chunk : q.len;
   if (j0 >= q.len && at.chunk > 0) return;
+  if (threadIdx.x < 64) lost[threadIdx.x] = 0;  // (set behind the last tile; without a tile there is nothing to walk again)
   float carry[V];  // a_t g_t of the token behind
   if (maps) {
     const int last = q.len > 0 ? (int)((q.len - 1) / a.chunk) : 0;
@@ -532,6 +731,9 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_backward_kernel(ScanArg
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = g_last && at.active ? g_last[sc + v] : 0.0f;
   }
+  float trace = 0.0f;  // NaN once something is not finite
+#pragma unroll
+  for (int v = 0; v < V; ++v) trace = __builtin_fmaf(carry[v], 0.0f, trace);
   const int64_t sx = q.dir * ldx, sf = q.dir * ldf, sy = q.dir * ldgy;
   const TileRows<T, V> tx(at, q, ldx), tf(at, q, ldf), ty(at, q, ldgy), tgx(at, q, ldgx), tgf(at, q, ldgf);
   const int64_t last_tile = j1 > j0 ? j0 + (j1 - j0 - 1) / tile * tile : j0 - tile;
@@ -632,6 +834,8 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_backward_kernel(ScanArg
         }
       }
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v) trace = __builtin_fmaf(h[v], 0.0f, __builtin_fmaf(c[v], 0.0f, trace));
     if (at.group == 0) {  // what goes back into the tile in front
 #pragma unroll
       for (int v = 0; v < V; ++v) ends[turn][at.slot + v] = carry[v] = c[v];
@@ -641,6 +845,14 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_backward_kernel(ScanArg
   for (int64_t jt = last_tile; jt >= j0; jt -= tile) {
     if (a.whole && jt + tile <= j1) one_tile(std::true_type{}, jt);
     else one_tile(std::false_type{}, jt);
+  }
+  if (__builtin_expect(trace != 0.0f, 0)) lost[at.slot / V] = 1;
+  __syncthreads();
+  if (__builtin_expect(at.group == 0 && at.active && lost[at.slot / V], 0)) {
+    float back[V];
+    sure_walk_back<T, V>(own_arguments<TileBackArgs<T>>(), &lds[0][0][0], back);
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = back[v];
   }
   if (g_h0 && at.chunk == 0 && at.group == 0 && at.active) {
 #pragma unroll

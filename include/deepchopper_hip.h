@@ -450,7 +450,8 @@ int dc_token_logprobs_backward(void* stream, const void* d_logits, int32_t dtype
 
 /* Gated linear recurrence over every channel of every sequence:
  *   a_t = sigmoid(f_t)    h_t = a_t h_(t-1) + (1 - a_t) x_t    y_t = h_t,   t along the sequence, or from its end (reverse)
- *  d_x, d_f   : [n_tokens, n_channels]; a gate of +inf keeps the state whatever x holds (padding)
+ *  d_x, d_f   : [n_tokens, n_channels]; a gate of +inf keeps the state whatever x holds (padding).  Weights a, 1 - a below
+ *               2^-126 are 0, but an infinite state (or gradient) stays infinite until it meets the other infinity: NaN
  *  d_begin, d_end: int64[n_seqs] on the device, sequence s = tokens [begin[s], end[s]) (offsets of a packed batch: pass
  *               offsets and offsets + 1), which may not overlap, or both NULL: n_seqs dense sequences of max_len tokens
  *  max_len    : no sequence is longer (host value: it shapes the launch)

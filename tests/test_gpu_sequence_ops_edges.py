@@ -16,6 +16,20 @@ def env(hip_lib):
     return torch, ops
 
 
+HALF_STEP = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
+TINY = {"float32": 2.0 ** -126, "float16": 2.0 ** -25, "bfloat16": 2.0 ** -126}  # half the smallest step (fp32 results below 2^-126 may be flushed)
+
+
+def check(name, got, want, bound):
+    """Off by no more than the bound for 32 bits and half a step of the output's type; what is not finite has to be the same."""
+    dt = str(got.dtype).replace("torch.", "")
+    g = host(got).reshape(want.shape)
+    with np.errstate(invalid="ignore"):
+        off = np.abs(g - want) - (bound + HALF_STEP[dt] * (np.abs(want) + bound) + TINY[dt])
+        right = np.where(np.isfinite(want), off <= 0, (g == want) | (np.isnan(g) & np.isnan(want)))
+    assert right.all(), f"{name}: {(~right).sum()} of {want.size} values off, first at {tuple(np.argwhere(~right)[0])}: {g[~right][:4]} for {want[~right][:4]}"
+
+
 def host(t):
     return t.detach().double().cpu().numpy()
 
@@ -99,3 +113,69 @@ def test_gated_scan_refused_sequences_leave_a_given_out(env):
     out = torch.full((100, 8), 5.0, device="cuda")
     r = ops.gated_scan(x, f, offsets=torch.tensor([10, 30, 90]).cuda(), max_len=20, out=out)
     assert (out[:10] == 5).all() and (out[30:] == 5).all() and (out[10:30] != 5).any(1).all() and torch.isnan(r["h_last"][1]).all()
+
+
+# ------------------------------------------------------------------------------------------
+# gated_scan: the end of fp32's range
+# ------------------------------------------------------------------------------------------
+def scan_against_the_definition(torch, ops, x, f, lengths, h0, gy, gl, reverse):
+    from oracle import sequence_ref as ref
+
+    ends = np.cumsum(lengths)
+    kw = dict(offsets=torch.tensor([0] + list(ends)).cuda(), max_len=max(lengths), h0=h0, reverse=reverse)
+    got = ops.gated_scan(x, f, save=True, **kw)
+    got.update(ops.gated_scan_backward(x, f, got["saved"], gy, grad_h_last=gl, **kw))
+    with np.errstate(invalid="ignore"):
+        want, bound = ref.gated_scan(host(x), host(f), [(int(e - n), int(e)) for e, n in zip(ends, lengths)], host(h0), reverse, host(gy), host(gl))
+    for name in want:
+        check(name, got[name], want[name], bound[name])
+    return got, want
+
+
+# token by token; tiles; whole tiles; chunks of one and of two channels a lane; narrow rows
+SIZES = [([7, 16, 1, 0], 33), ([300, 17, 0], 48), ([1000, 130], 128), ([9001, 0, 700], 64), ([5000], 130), ([3000, 40], 5)]
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("lengths,c", SIZES)
+def test_gated_scan_of_the_largest_numbers(env, lengths, c, dtype, reverse):
+    """States between inputs of the type's largest and lowest values are finite: x - h is not.  (Gradients of 0.02, so that theirs are too.)"""
+    torch, ops = env
+    gen = torch.Generator().manual_seed(54)
+    n, k, most = sum(lengths), len(lengths), torch.finfo(getattr(torch, dtype)).max
+
+    def huge(*shape):
+        t = torch.rand(shape, generator=gen) * 0.5 + 0.5
+        t[torch.rand(shape, generator=gen) < 0.3] = 1.0
+        return t * torch.where(torch.rand(shape, generator=gen) < 0.5, -most, most)
+
+    x, h0 = huge(n, c).to(getattr(torch, dtype)).cuda(), huge(k, c).cuda()
+    x[: n // 3, 0] = -most  # a column that stays at the lowest value for long
+    f = randn(torch, gen, n, c, dtype=dtype, scale=2.0)
+    f[:, -1] += 5.0  # ... and one of a long memory
+    gy, gl = randn(torch, gen, n, c, dtype=dtype, scale=0.005), randn(torch, gen, k, c, scale=0.02)
+    got, want = scan_against_the_definition(torch, ops, x, f, lengths, h0, gy, gl, reverse)
+    assert np.isfinite(want["y"]).all() and torch.isfinite(got["y"]).all()
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("lengths,c", SIZES)
+def test_gated_scan_infinities_go_as_the_definition_says(env, lengths, c, dtype, reverse):
+    """An infinite input or state, or one of either sign and then NaN, from there on; infinite gradients; other channels as ever."""
+    torch, ops = env
+    gen = torch.Generator().manual_seed(55)
+    n, k = sum(lengths), len(lengths)
+    x, f, gy = (randn(torch, gen, n, c, dtype=dtype) for _ in range(3))
+    h0, gl = randn(torch, gen, k, c), randn(torch, gen, k, c)
+    x[n // 2, 0] = float("inf")
+    x[n // 3, 1] = float("-inf")
+    x[2 * n // 3, 1] = float("inf")
+    h0[:, 2] = float("inf")
+    gy[n // 2, 3] = float("-inf")
+    gl[:, 4] = float("inf")
+    x[n // 4, c - 1] = float("nan")
+    f[:, 0] -= 6.0  # strongly forgetting
+    f[:, 2] += 20.0  # keeping: weights below fp32's last digit
+    scan_against_the_definition(torch, ops, x, f, lengths, h0, gy, gl, reverse)
