@@ -32,8 +32,6 @@ struct NormArgs {
   int32_t serial;
 };
 
-__device__ __forceinline__ float sigmoid(float x) { return fast_rcp(1.0f + fast_exp2(-x * kLog2e)); }
-
 // One row's columns of this thread: K vectors of V, 256 * n_waves apart.  Elements beyond the width are 0 and not stored.
 template <int K>
 struct Part {
@@ -131,7 +129,8 @@ __device__ __forceinline__ void widen(const RawPart<T, K>& p, Part<K>& out) {
 #pragma unroll
     for (int i = 0; i < V; ++i) out.v[k][i] = (float)p.r[k][i];
 }
-// The gate's activation, in place; with `slope`, its derivative.
+// The gate's activation, in place; with `slope`, its derivative.  With e = exp(-x) and s = 1 / (1 + e), 1 - s is e s, which keeps its digits
+// where s is next to 1 (and is 1 where e is infinite).
 template <int K>
 __device__ __forceinline__ void activate(const NormArgs& a, Part<K>& g, Part<K>* slope) {
   if (a.act == DC_ACT_IDENTITY) {
@@ -148,8 +147,11 @@ __device__ __forceinline__ void activate(const NormArgs& a, Part<K>& g, Part<K>*
   for (int k = 0; k < K; ++k) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float x = g.v[k][i], s = sigmoid(x);
-      if (slope) slope->v[k][i] = s * (silu ? __builtin_fmaf(x, 1.0f - s, 1.0f) : 1.0f - s);
+      const float x = g.v[k][i], e = fast_exp2(-x * kLog2e), s = fast_rcp(1.0f + e);
+      if (slope) {
+        const float rest = __builtin_fminf(e * s, 1.0f);
+        slope->v[k][i] = s * (silu ? __builtin_fmaf(x, rest, 1.0f) : rest);
+      }
       g.v[k][i] = silu ? x * s : s;
     }
   }

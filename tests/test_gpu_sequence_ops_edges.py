@@ -179,3 +179,36 @@ def test_gated_scan_infinities_go_as_the_definition_says(env, lengths, c, dtype,
     f[:, 0] -= 6.0  # strongly forgetting
     f[:, 2] += 20.0  # keeping: weights below fp32's last digit
     scan_against_the_definition(torch, ops, x, f, lengths, h0, gy, gl, reverse)
+
+
+# ------------------------------------------------------------------------------------------
+# block_norm
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("width", [8, 64, 250, 600])
+def test_block_norm_slope_of_gates_that_are_all_but_open(env, width, dtype, act):
+    """r' = act(gate) alone: its gradient is s (1 - s), or s (1 + x (1 - s)), with relative accuracy also where s rounds to 1.
+
+    exp(-x) by a rounded x log2(e) (1.5 |x| half steps) and a one-ulp exp2 (2), 1 + e and a one-ulp reciprocal (3), e s (1), the product of
+    the two (1), each error but the last ones in both factors: (1.5 |x| + 12) half steps; silu's x (1 - s) has another 1.5 |x|."""
+    torch, ops = env
+    from oracle.sequence_ref import U
+
+    rows = 40
+    x = torch.linspace(-80.0, 80.0, rows * width).reshape(rows, width)
+    x[0] = torch.linspace(-30.0, 30.0, width)
+    x[1, :6] = torch.tensor([12.0, 15.0, 17.0, 30.0, -12.0, 0.0])
+    x[2, :2] = torch.tensor([float("inf"), torch.finfo(torch.float32).min / 2])
+    gate = x.to(getattr(torch, dtype)).cuda()
+    one = torch.ones((rows, width), dtype=gate.dtype, device="cuda")
+    if act == "silu":
+        gate[2, 0] = 80.0  # (x (1 - s) of an infinite x is no number)
+    got = ops.block_norm_backward(one, None, gate, post=False, gate_act=act, grad_residual=one)["grad_gate"]
+    x = host(gate)
+    with np.errstate(over="ignore", invalid="ignore"):
+        s, rest = 1 / (1 + np.exp(-x)), 1 / (1 + np.exp(x))
+        want = s * rest if act == "sigmoid" else s * (1 + x * rest)
+        bound = (1.5 * np.abs(x) + 12) * U * np.abs(want) if act == "sigmoid" else (3 * np.abs(x) + 14) * U * s * (1 + np.abs(x) * rest)
+    bound = np.where(np.isfinite(x), np.minimum(bound, 1.0), 0.0)  # (beyond 88 the slope is below fp32's normal numbers)
+    check("grad_gate", got, want, bound)
