@@ -51,10 +51,21 @@ struct RowStats {
 };
 __device__ __forceinline__ float log_prob(const RowStats& r, float z) { return r.m == -INFINITY ? -INFINITY : (z - r.m) - r.log_sum; }
 
-// dz without the given token's + g
+// dz of the other classes
 __device__ __forceinline__ float grad_at(const RowStats& r, float z, float g, float h) {
   const float lp = (z - r.m) - r.log_sum, p = fast_exp2(lp * kLog2e);
   return p == 0.0f ? 0.0f : -p * __builtin_fmaf(h, lp + r.entropy, g);
+}
+// dz of the given one, g (1 - p) - h p (lp + H): for p next to 1 its 1 - p is the series of -expm1(lp) (below 1/4 to 2^-29), not a difference
+__device__ __forceinline__ float grad_of_given(const RowStats& r, float z, float g, float h) {
+  const float lp = (z - r.m) - r.log_sum, p = fast_exp2(lp * kLog2e), u = -lp;
+  float rest = __builtin_fmaf(u, 1.0f / 5040, -1.0f / 720);
+  rest = __builtin_fmaf(u, rest, 1.0f / 120);
+  rest = __builtin_fmaf(u, rest, -1.0f / 24);
+  rest = __builtin_fmaf(u, rest, 1.0f / 6);
+  rest = __builtin_fmaf(u, rest, -0.5f);
+  rest = __builtin_fmaf(u, rest, 1.0f) * u;
+  return p == 0.0f ? g : __builtin_fmaf(g, u < 0.25f ? rest : 1.0f - p, -h * p * (lp + r.entropy));
 }
 
 // what a row's gradient is: as the formula says, zeros (skipped, or nothing is possible), or NaN (a token outside the classes)
@@ -235,14 +246,17 @@ __global__ __launch_bounds__(256) void few_classes_backward_kernel(const T* logi
       r = few_stats<E>(f, bits);
     }
     const RowGrad what = row_grad(skip, r, g_logprob && !(t >= 0 && t < n));
+    float given = 0.0f;
+#pragma unroll
+    for (int k = 0; k < E; ++k) given = f.c[k] == t ? f.z[k] : given;
+    given = grad_of_given(r, given, g, h);
 #pragma unroll
     for (int k = 0; k < E / W; ++k) {
       const int c = ((k << bits) + lane) * W;
       float v[W];
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        v[w] = what == kZeros ? 0.0f : what == kNans ? __builtin_nanf("") : grad_at(r, f.z[k * W + w], g, h);
-        if (what == kFormula && c + w == t) v[w] += g;
+        v[w] = what == kZeros ? 0.0f : what == kNans ? __builtin_nanf("") : c + w == t ? given : grad_at(r, f.z[k * W + w], g, h);
       }
       T* o = out + i * ld_out + c;
       if (c + W <= n) {
@@ -598,9 +612,12 @@ __global__ __launch_bounds__(256) void many_classes_backward_kernel(const T* log
 #pragma unroll
         for (int w = 0; w < W; ++w) d[w] = grad_at(r, (float)raw[q][w], g, h);
         if (t >= c && t < c + W) {
+          float given = 0.0f;
 #pragma unroll
-          for (int w = 0; w < W; ++w)
-            if (c + w == t) d[w] += g;
+          for (int w = 0; w < W; ++w) given = c + w == t ? (float)raw[q][w] : given;
+          given = grad_of_given(r, given, g, h);
+#pragma unroll
+          for (int w = 0; w < W; ++w) d[w] = c + w == t ? given : d[w];
         }
       }
       store_vec<W>(o + c, d);
@@ -610,7 +627,7 @@ __global__ __launch_bounds__(256) void many_classes_backward_kernel(const T* log
     for (int e = 0; e < 2; ++e) {
       if (!(e ? last : first)) continue;
       const int c = (e ? tail_at : 0) + threadIdx.x;
-      o[c] = (T)(what == kFormula ? grad_at(r, (float)row[c], g, h) + (c == t ? g : 0.0f) : flat);
+      o[c] = (T)(what != kFormula ? flat : c == t ? grad_of_given(r, (float)row[c], g, h) : grad_at(r, (float)row[c], g, h));
     }
   }
 }

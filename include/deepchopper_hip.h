@@ -431,7 +431,9 @@ int dc_model_profile_stages(dc_model* m, char* buf, int32_t buf_len);
  *  d_top_ids, d_top_logprob: int32 / float[n_rows, n_top]: the n_top (<= n_classes, <= DC_MAX_TOP) classes of the largest
  *                 logits in descending order, ties to the lower class, and their log probabilities; n_top = 0: NULL.
  *  Logits of -inf are classes that cannot be: probability 0.  A row of nothing else has log probabilities -inf, entropy 0 and
- *  zero gradients.  A NaN or +inf in a row makes its log probabilities and entropy NaN (NaN sorts as the largest). */
+ *  zero gradients, whatever its token.  A NaN or +inf in a row makes its log probabilities and entropy NaN (NaN sorts as the
+ *  largest).  Below DC_STATS_FROM classes the log probability of an almost sure class, and 1 - p of its gradient, keep their
+ *  relative accuracy; from there on S holds that class's 1 and they are accurate to a few 2^-24 of 1. */
 int dc_token_logprobs(void* stream, const void* d_logits, int32_t dtype, int64_t n_rows, int32_t n_classes,
                       int64_t row_stride, const void* d_tokens, int32_t token_type, int64_t ignore_token, int32_t n_top,
                       float* d_logprob, float* d_entropy, float* d_stats, int32_t* d_top_ids, float* d_top_logprob,

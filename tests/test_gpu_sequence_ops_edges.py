@@ -212,3 +212,37 @@ def test_block_norm_slope_of_gates_that_are_all_but_open(env, width, dtype, act)
         bound = (1.5 * np.abs(x) + 12) * U * np.abs(want) if act == "sigmoid" else (3 * np.abs(x) + 14) * U * s * (1 + np.abs(x) * rest)
     bound = np.where(np.isfinite(x), np.minimum(bound, 1.0), 0.0)  # (beyond 88 the slope is below fp32's normal numbers)
     check("grad_gate", got, want, bound)
+
+
+# ------------------------------------------------------------------------------------------
+# token_logprobs
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("classes", [2, 3, 4, 5, 16, 50, 100, 300, 512])
+def test_token_logprobs_gradient_of_a_sure_row_keeps_its_digits(env, classes, dtype):
+    """A given class 5 to 70 above the others: its gradient is g (1 - p), not 0, and a row's gradients add up to 0.
+
+    log p keeps its digits to (2 gap + 8) half steps as a log1p of a sum (of up to 16 terms a lane and 5 steps over lanes: 21 more), the
+    series of 1 - p to 8 and the product to 1.  Classes a little above give the other form of 1 - p: p is off by (2 |log p| + 4) half steps
+    besides log p's 30, and at least a fifth of 1 is left: 5 times that."""
+    torch, ops = env
+    from oracle.sequence_ref import U
+
+    gen = torch.Generator().manual_seed(56)
+    gaps = torch.tensor([70.0, 60.0, 40.0, 25.0, 16.0, 9.0, 5.0, 3.0, 2.0, 1.0, 0.5])
+    z = torch.rand((len(gaps), classes), generator=gen) * -2 - gaps[:, None] - np.log(classes)
+    t = torch.randint(0, classes, (len(gaps),), generator=gen)
+    z[torch.arange(len(gaps)), t] = 0.0
+    z = z.to(getattr(torch, dtype)).cuda()
+    g = torch.linspace(0.5, 2.0, len(gaps))
+    got = ops.token_logprobs_backward(z, t.cuda(), None, g.cuda())
+    zd, rows = host(z), np.arange(len(gaps))
+    e = np.exp(zd)
+    others = e.sum(1) - 1 if classes < 2 else np.array([np.delete(e[i], int(t[i])).sum() for i in rows])
+    want = g.double().numpy() * others / (1 + others)
+    gap = -np.sort(zd, 1)[:, -2]
+    bound = np.where(others < 0.25, 2 * gap + 40, 5 * 40) * U * want
+    check("given", got[torch.arange(len(gaps)), t.cuda()], want, bound)
+    if dtype == "float32":
+        total = host(got).sum(1)  # the other classes' gradients -g p_j are as accurate, and each is rounded once
+        assert (np.abs(total) <= 2 * (bound + (2 * (gap + 2 + np.log(classes)) + 40) * U * want)).all()
