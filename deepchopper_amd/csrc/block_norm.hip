@@ -554,17 +554,18 @@ __global__ __launch_bounds__(THREADS, waves_a_simd(sizeof(R), K, F, THREADS)) vo
 
 struct SumOut {
   float* p[5];
+  int32_t n_parts[5];  // 0: a vector that the call did not use
 };
 
 // 32 columns of one vector, the parts divided over 32 rows of threads.
-__global__ __launch_bounds__(1024) void block_norm_sums_kernel(const float* __restrict__ sums, int32_t n_parts, int32_t width, SumOut out) {
+__global__ __launch_bounds__(1024) void block_norm_sums_kernel(const float* __restrict__ sums, int32_t width, SumOut out) {
   __shared__ float lds[32][33];
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, k = blockIdx.y;
   if (!out.p[k]) return;
   float s = 0.0f;
   if (c < width) {
 #pragma unroll 8
-    for (int i = part; i < n_parts; i += 32) s += sums[((int64_t)i * 5 + k) * width + c];
+    for (int i = part; i < out.n_parts[k]; i += 32) s += sums[((int64_t)i * 5 + k) * width + c];
   }
   lds[part][lane] = s;
   __syncthreads();
@@ -710,7 +711,8 @@ extern "C" int dc_block_norm_backward(void* stream, int32_t dtype, int32_t resid
     }
     if (any) {
       block_norm_sums_kernel<<<dim3((width + 31) / 32, 5), dim3(1024), 0, as_stream(stream)>>>(
-          (const float*)d_workspace, grid, width, SumOut{{d_grad_scale, d_grad_post_w, d_grad_post_b, d_grad_pre_w, d_grad_pre_b}});
+          (const float*)d_workspace, width,
+          SumOut{{d_grad_scale, d_grad_post_w, d_grad_post_b, d_grad_pre_w, d_grad_pre_b}, {grid, post_norm ? grid : 0, post_norm ? grid : 0, grid, grid}});
       DC_LAUNCH_CHECK();
     }
     return DC_OK;

@@ -504,7 +504,7 @@ int dc_block_norm(void* stream, int32_t dtype, int32_t residual_dtype, int64_t n
 /* Its backward pass: the same inputs (d_residual as it was BEFORE the forward call), and the gradients of r' and n
  * (either or NULL: zero).  r', the norms' statistics and u are computed again from the inputs.
  *  d_grad_y, d_grad_gate, d_grad_residual: dense, or NULL;  d_grad_scale, d_grad_*_w, d_grad_*_b: float[width], or NULL
- *  (summed over the rows in a fixed order). */
+ *  (summed over the rows in a fixed order; zeros for a vector that the forward call did not use). */
 int dc_block_norm_backward(void* stream, int32_t dtype, int32_t residual_dtype, int64_t n_rows, int32_t width, int32_t kind,
                            float eps, const void* d_y, int64_t y_stride, const void* d_gate, int64_t gate_stride,
                            int32_t gate_act, const void* d_residual, int64_t residual_stride, const float* d_scale,

@@ -214,6 +214,30 @@ def test_block_norm_slope_of_gates_that_are_all_but_open(env, width, dtype, act)
     check("grad_gate", got, want, bound)
 
 
+@pytest.mark.parametrize("width", [64, 600])
+@pytest.mark.parametrize("with_y,post,with_normed", [(True, 0, True), (True, 1, False), (False, 1, True), (True, 0, False)])
+def test_block_norm_gradients_of_vectors_that_were_not_used_are_zero(env, width, with_y, post, with_normed):
+    """The C entry with all five vectors' pointers: without a norm behind the block, without the next block's, without a block."""
+    torch, ops = env
+    from deepchopper_amd import _lib
+
+    gen = torch.Generator().manual_seed(57)
+    rows = 70
+    y, r, gr, gn = (randn(torch, gen, rows, width) for _ in range(4))
+    w = [randn(torch, gen, width, shift=1.0) for _ in range(4)]
+    out = [torch.full((width,), 77.0, device="cuda") for _ in range(5)]
+    grads = [torch.empty((rows, width), device="cuda") for _ in range(2)]
+    L = _lib.lib()
+    nb = L.dc_block_norm_workspace(rows, width, 0)
+    ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    at = lambda t, used=True: t.data_ptr() if used else None  # noqa: E731
+    _lib.check(L.dc_block_norm_backward(torch.cuda.current_stream().cuda_stream, 0, 0, rows, width, 0, 1e-5, at(y, with_y), width, None, 0, 0, at(r), width,
+                                        at(w[0]), post, at(w[1]), at(w[2]), at(w[3]), at(gr), width, at(gn, with_normed), width, at(grads[0], with_y), None,
+                                        at(grads[1]), *(t.data_ptr() for t in out), ws.data_ptr(), nb))
+    for t, used in zip(out, (with_y, with_y and post, with_y and post, with_normed, with_normed)):
+        assert (t != 0).any() and (t != 77).all() if used else (t == 0).all()
+
+
 # ------------------------------------------------------------------------------------------
 # token_logprobs
 # ------------------------------------------------------------------------------------------
