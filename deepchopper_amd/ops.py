@@ -191,7 +191,8 @@ def summary_predict_dense(pred: torch.Tensor, labels: torch.Tensor, ignore_label
 
 
 # ------------------------------------------------------------------------------------------
-# sequence-layer and scoring operators.  None of them is recorded by torch's autograd: the gradients are the *_backward functions'.
+# sequence-layer and scoring operators.  None of them is recorded by torch's autograd: the gradients are the *_backward functions', and a call
+# whose inputs autograd would follow is refused.
 # ------------------------------------------------------------------------------------------
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _TOKEN_TYPES = {torch.int8: 0, torch.uint8: 1, torch.int32: 2, torch.int64: 3}
@@ -222,6 +223,14 @@ def _on(dev: int):
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
+
+
+def _not_recorded(name: str, *inputs: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled():
+        for t in inputs:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name}: an input requires gradients, but autograd does not record this operator: call it under torch.no_grad() or "
+                                 f"with detached tensors, and take the gradients from {name}_backward")
 
 
 def _like(dev: int, name: str, t: torch.Tensor | None, shape: tuple, dtype: torch.dtype) -> int | None:
@@ -281,6 +290,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     (labels of padding) are not read and give 0, alternatives -1.  Returns dict(logprob f32 or None, entropy f32 or None,
     top_ids i32, top_logprob f32 [..., n_top] or None, stats: what `token_logprobs_backward` needs (with `save`; None below STATS_FROM
     classes))."""
+    _not_recorded("token_logprobs", logits)
     dev = _device_of("logits", logits)
     ptr, stride = _rows(dev, "logits", logits)
     lead, n_classes, dtype = logits.shape[:-1], logits.shape[-1], logits.dtype
@@ -354,6 +364,7 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, *, offsets: torch.Tensor | None
     tokens of no sequence, which are zero otherwise.  `max_len`: no sequence is longer (found on the host, with a wait, where it is not
     given).  A sequence that is, or that leaves the tokens, is refused: NaN in its row of h_last and, with `offsets`, in its rows of y; with
     `begin` / `end` or a given `out` those stay as tokens of no sequence.  Returns dict(y, h_last, saved: for `gated_scan_backward`, with `save`)."""
+    _not_recorded("gated_scan", x, f, h0)
     dev = _device_of("x", x)
     xp, xs = _rows(dev, "x", x)
     shape, dtype, device = x.shape, x.dtype, x.device
@@ -430,6 +441,7 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None = None, gat
     front of the next (the last block); y None: the first norm of a model; residual None: r' is the block's output alone.  Norms are
     "layer" or "rms", gates "identity", "sigmoid" or "silu"; weights, biases and `scale` are float32[width].  `dtype`: of n where y is
     None (default: the residual's); `out`: where r' goes (`residual` itself: in place).  Returns dict(residual: r', normed: n or None)."""
+    _not_recorded("block_norm", y, residual, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
     ref = _norm_ref(y, residual)
     dev = _device_of("residual" if y is None else "y", ref)
     k, act = _norm_codes(kind, gate_act)
