@@ -314,6 +314,14 @@ __device__ __forceinline__ RowStats finish(const Running& r) {
   return {r.m == -INFINITY ? 0.0f : r.m, log_sum, log_sum - kLn2 * r.u / r.s};
 }
 
+// What the lanes of a wavefront have stored to LDS, all of them read from here on.  (A wavefront's LDS accesses are carried out in order: this
+// keeps the compiler from changing it.)
+__device__ __forceinline__ void wave_meets() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Candidates of one wavefront in LDS: (key, ~class) as one number, larger is better.
 struct Candidates {
   uint64_t* list;  // [128]
@@ -334,14 +342,14 @@ struct Candidates {
     }
     if (mask >> (threadIdx.x & 63) & 1) list[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = cand;
     n += __popcll(mask);
-    __builtin_amdgcn_wave_barrier();
+    wave_meets();
   }
 
   // the k best, in order, to the front of the list: everyone counts how many are better than its one or two
   __device__ void rank() {
     if (n == ranked) return;
     const int lane = threadIdx.x & 63;
-    __builtin_amdgcn_wave_barrier();
+    wave_meets();
     const uint64_t a = lane < n ? list[lane] : 0, b = lane + 64 < n ? list[lane + 64] : 0;
     int ra = 0, rb = 0;
     if (n <= 64) {
@@ -354,10 +362,10 @@ struct Candidates {
         ra += o > a, rb += o > b;
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_meets();
     if (lane < n && ra < k) list[ra] = a;
     if (lane + 64 < n && rb < k) list[rb] = b;
-    __builtin_amdgcn_wave_barrier();
+    wave_meets();
     if (n >= k) {
       n = k;
       worst = list[k - 1];
@@ -531,7 +539,7 @@ __global__ __launch_bounds__(256) void many_classes_kernel(const T* __restrict__
         if (lane < n_top) sl.best[unit * n_top + lane] = lane < best.n ? best.list[lane] : 0;
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_meets();
   }
 }
 
@@ -569,7 +577,7 @@ __global__ __launch_bounds__(64) void join_slices_kernel(const T* __restrict__ l
       best.rank();
     }
     write_row(out, i, logits + i * ld, n, t, tok.p != nullptr, finish(r), n_top, lds);
-    __builtin_amdgcn_wave_barrier();
+    wave_meets();
   }
 }
 
