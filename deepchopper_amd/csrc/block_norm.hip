@@ -623,8 +623,9 @@ int check_norm(int32_t dtype, int32_t residual_dtype, int64_t n_rows, int32_t wi
   return DC_OK;
 }
 
-// calls f with the element types, the vectors a lane and whether a row takes several wavefronts
-template <typename F>
+// calls f with the element types, the vectors a lane and whether a row takes several wavefronts.  (Of the forms only those that row_plan
+// gives: two vectors a lane forward in one wavefront or more, backward only beyond 16; one of 5 to 16 wavefronts only backward.)
+template <bool BACK, typename F>
 int with_row(int32_t dtype, int32_t residual_dtype, const RowPlan& p, F&& f) {
   return with_dtype(dtype, [&](auto t) {
     auto g = [&](auto r) {
@@ -635,9 +636,15 @@ int with_row(int32_t dtype, int32_t residual_dtype, const RowPlan& p, F&& f) {
       using Small = std::integral_constant<int, 256>;
       using Large = std::integral_constant<int, 1024>;
       if (p.n_waves == 1 && p.lane_bits < 6) return f(t, r, One{}, std::integral_constant<Form, kSub>{}, Small{});
-      if (p.n_waves == 1) return p.k == 1 ? f(t, r, One{}, Wave{}, Small{}) : f(t, r, Two{}, Wave{}, Small{});
-      if (p.n_waves <= 4) return p.k == 1 ? f(t, r, One{}, Team{}, Small{}) : f(t, r, Two{}, Team{}, Small{});
-      return p.k == 1 ? f(t, r, One{}, Team{}, Large{}) : f(t, r, Two{}, Team{}, Large{});
+      if constexpr (BACK) {
+        if (p.n_waves == 1) return f(t, r, One{}, Wave{}, Small{});
+        if (p.n_waves <= 4) return f(t, r, One{}, Team{}, Small{});
+        return p.k == 1 ? f(t, r, One{}, Team{}, Large{}) : f(t, r, Two{}, Team{}, Large{});
+      } else {
+        if (p.n_waves == 1) return p.k == 1 ? f(t, r, One{}, Wave{}, Small{}) : f(t, r, Two{}, Wave{}, Small{});
+        if (p.n_waves <= 4) return p.k == 1 ? f(t, r, One{}, Team{}, Small{}) : f(t, r, Two{}, Team{}, Small{});
+        return f(t, r, Two{}, Team{}, Large{});
+      }
     };
     return residual_dtype == dtype ? g(t) : g(f32{});
   });
@@ -667,7 +674,7 @@ extern "C" int dc_block_norm(void* stream, int32_t dtype, int32_t residual_dtype
   const int groups = p.n_waves > 1 ? p.threads / 64 / p.n_waves : p.threads >> p.lane_bits;
   const int64_t need = (n_rows + groups - 1) / groups;
   const int grid = (int)(need < 4096 ? need : 4096);
-  return with_row(dtype, residual_dtype, p, [&](auto t, auto r, auto k, auto form, auto threads) {
+  return with_row<false>(dtype, residual_dtype, p, [&](auto t, auto r, auto k, auto form, auto threads) {
     using T = decltype(t);
     using R = decltype(r);
     block_norm_kernel<T, R, decltype(k)::value, decltype(form)::value, decltype(threads)::value><<<dim3(grid), dim3(p.threads), 0, as_stream(stream)>>>(
@@ -697,7 +704,7 @@ extern "C" int dc_block_norm_backward(void* stream, int32_t dtype, int32_t resid
   const int groups = p.n_waves > 1 ? p.threads / 64 / p.n_waves : p.threads >> p.lane_bits;
   const int grid = parts_of(n_rows, width, residual_dtype);
   const bool any = d_grad_scale || d_grad_post_w || d_grad_post_b || d_grad_pre_w || d_grad_pre_b;
-  return with_row(dtype, residual_dtype, p, [&](auto t, auto r, auto k, auto form, auto threads) {
+  return with_row<true>(dtype, residual_dtype, p, [&](auto t, auto r, auto k, auto form, auto threads) {
     using T = decltype(t);
     using R = decltype(r);
     if (grid > 0) {
