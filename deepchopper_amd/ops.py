@@ -265,6 +265,26 @@ def _rows(dev: int, name: str, t: torch.Tensor | None, shape: torch.Size | None 
     return t.data_ptr(), dims[-1][1] if dims else size[-1]
 
 
+def _apart(name: str, out: torch.Tensor, out_rows: tuple[int, int], other_name: str, other: torch.Tensor | None, rows: tuple[int | None, int],
+           same: bool = False) -> None:
+    """Refuses an output given by the caller that shares elements with an input: a kernel would read what another workgroup has written.
+    `rows` as `_rows` returned them; `same`: the output may be that input itself, row for row."""
+    if other is None or not out.numel() or out_rows[1] < out.shape[-1]:  # (rows that overlap among themselves are refused by the library)
+        return
+    width, n = out.shape[-1], out.numel() // out.shape[-1]
+    ea, eb = out.element_size(), other.element_size()
+    a, sa, b, sb = out_rows[0], out_rows[1] * ea, rows[0], rows[1] * eb
+    wa, wb = width * ea, width * eb
+    if a >= b + (n - 1) * sb + wb or b >= a + (n - 1) * sa + wa or (same and a == b and sa == sb and ea == eb):
+        return
+    if n > 1 and sa == sb and wa <= (b - a) % sa <= sa - wb:  # other columns of the same rows
+        return
+    starts, others = a + sa * np.arange(n), b + sb * np.arange(n)
+    k = np.searchsorted(starts, others, side="right")  # rows k - 1 and k of the output lie on either side of an input's row's start
+    if ((k > 0) & (starts[np.maximum(k, 1) - 1] + wa > others)).any() or ((k < n) & (starts[np.minimum(k, n - 1)] < others + wb)).any():
+        raise ValueError(f"{name}: shares elements with {other_name}")
+
+
 def _new_like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """A dense tensor of `t`'s shape and device (`empty_like` takes half the time of `empty`)."""
     return torch.empty_like(t) if t.dtype is dtype and t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
@@ -360,8 +380,8 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, *, offsets: torch.Tensor | None
 
     x, f [n_seqs, length, n_channels] dense, or [n_tokens, n_channels] with the sequences at `offsets` int64[n_seqs + 1], or at
     `begin` / `end` int64[n_seqs] (left-padded rows: first column and end of each).  `h0` f32[n_seqs, n_channels] state to start from; `reverse`: from
-    the sequences' ends.  `h_last` may be given (`h0` itself: a state kept in place while bases stream in); `out` keeps what stands in
-    tokens of no sequence, which are zero otherwise.  `max_len`: no sequence is longer (found on the host, with a wait, where it is not
+    the sequences' ends.  `h_last` may be given (`h0` itself: a state kept in place while bases stream in); `out` (apart from x and f) keeps
+    what stands in tokens of no sequence, which are zero otherwise.  `max_len`: no sequence is longer (found on the host, with a wait, where it is not
     given).  A sequence that is, or that leaves the tokens, is refused: NaN in its row of h_last and, with `offsets`, in its rows of y; with
     `begin` / `end` or a given `out` those stay as tokens of no sequence.  Returns dict(y, h_last, saved: for `gated_scan_backward`, with `save`)."""
     _not_recorded("gated_scan", x, f, h0)
@@ -374,10 +394,16 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, *, offsets: torch.Tensor | None
     zero_rest = out is None and offsets is not None  # (dense sequences cover every token)
     if out is None:
         out = _new_like(x, dtype) if begin is None else torch.zeros(shape, dtype=dtype, device=device)
-    yp, ys = _rows(dev, "out", out, shape, dtype)
+        yp, ys = _rows(dev, "out", out, shape, dtype)
+    else:
+        yp, ys = _rows(dev, "out", out, shape, dtype)
+        _apart("out", out, (yp, ys), "x", x, (xp, xs))
+        _apart("out", out, (yp, ys), "f", f, (fp, fs))
     if h_last is None:
         h_last = torch.empty_like(h0) if h0 is not None else x.new_empty((seqs, c), dtype=torch.float32)
     hp = _like(dev, "h_last", h_last, (seqs, c), torch.float32)
+    if h0p is not None and h0p != hp:
+        _apart("h_last", h_last, (hp, c), "h0", h0, (h0p, c))
     L = _lib.lib()
     saved = x.new_empty(L.dc_gated_scan_saved(n, c), dtype=torch.float32) if save else None
     nb = L.dc_gated_scan_workspace(n, c, seqs, longest) if longest > 1 else 0
@@ -440,7 +466,7 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None = None, gat
     y, gate [..., width] of one type, residual of that type or float32.  `post=False`: no norm behind the block; `pre=False`: none in
     front of the next (the last block); y None: the first norm of a model; residual None: r' is the block's output alone.  Norms are
     "layer" or "rms", gates "identity", "sigmoid" or "silu"; weights, biases and `scale` are float32[width].  `dtype`: of n where y is
-    None (default: the residual's); `out`: where r' goes (`residual` itself: in place).  Returns dict(residual: r', normed: n or None)."""
+    None (default: the residual's); `out`: where r' goes (an input of its type itself: in place).  Returns dict(residual: r', normed: n or None)."""
     _not_recorded("block_norm", y, residual, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
     ref = _norm_ref(y, residual)
     dev = _device_of("residual" if y is None else "y", ref)
@@ -458,9 +484,14 @@ def block_norm(y: torch.Tensor | None, residual: torch.Tensor | None = None, gat
     sc = _like(dev, "scale", scale, one, torch.float32)
     pw, pb = _like(dev, "post_weight", post_weight, one, torch.float32), _like(dev, "post_bias", post_bias, one, torch.float32)
     qw, qb = _like(dev, "pre_weight", pre_weight, one, torch.float32), _like(dev, "pre_bias", pre_bias, one, torch.float32)
+    given = out is not None
     if out is None and y is not None:
         out = _new_like(residual if residual is not None else y, res_dtype)
     op, os_ = _rows(dev, "out", out, shape, res_dtype)
+    if given:
+        _apart("out", out, (op, os_), "y", y, (yp, ys), same=True)
+        _apart("out", out, (op, os_), "gate", gate, (gp, gs), same=True)
+        _apart("out", out, (op, os_), "residual", residual, (rp, rs), same=True)
     normed = _new_like(ref, act_dtype) if pre else None
     with _on(dev):
         _lib.check(_lib.lib().dc_block_norm(

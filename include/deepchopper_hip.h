@@ -478,7 +478,7 @@ int64_t dc_gated_scan_saved(int64_t n_tokens, int32_t n_channels);
  *   dx_t = (1 - a_t) g_t    df_t = g_t (h_(t-1) - x_t) a_t (1 - a_t)    dh0 = a_0 g_0
  *  inputs as in the forward call, d_saved as it left it; d_grad_h_last or NULL; d_grad_h0 or NULL.
  *  The states between two tiles are computed again from d_saved in fp32 (y, rounded, is not read).
- *  d_grad_x, d_grad_f: [n_tokens, n_channels]; tokens of no sequence as in d_y. */
+ *  d_grad_x, d_grad_f: [n_tokens, n_channels], not overlapping the inputs; tokens of no sequence as in d_y. */
 int dc_gated_scan_backward(void* stream, int32_t dtype, const void* d_x, int64_t x_stride, const void* d_f, int64_t f_stride,
                            int64_t n_tokens, int32_t n_channels, const int64_t* d_begin, const int64_t* d_end,
                            int32_t n_seqs, int64_t max_len, int32_t reverse, const float* d_h0, const float* d_saved,
@@ -494,7 +494,8 @@ int dc_gated_scan_backward(void* stream, int32_t dtype, const void* d_x, int64_t
  *                   before r' is rounded
  *  d_y            : NULL: no block in front (r' = residual; the first norm of a model);  d_residual NULL: r' = scale * v
  *  d_scale, d_*_w : float[width] or NULL (ones);  d_*_b: float[width] or NULL (zeros)
- *  d_residual_out : or NULL (not stored); it may be d_residual itself;  d_normed: or NULL (no norm in front of a next block) */
+ *  d_residual_out : or NULL (not stored); it may be d_residual, d_y or d_gate itself (same address, stride and type), but not
+ *                   overlap an input otherwise;  d_normed: or NULL (no norm in front of a next block) */
 int dc_block_norm(void* stream, int32_t dtype, int32_t residual_dtype, int64_t n_rows, int32_t width, int32_t kind,
                   float eps, const void* d_y, int64_t y_stride, const void* d_gate, int64_t gate_stride, int32_t gate_act,
                   const void* d_residual, int64_t residual_stride, const float* d_scale, int32_t post_norm,

@@ -270,3 +270,53 @@ def test_token_logprobs_gradient_of_a_sure_row_keeps_its_digits(env, classes, dt
     if dtype == "float32":
         total = host(got).sum(1)  # the other classes' gradients -g p_j are as accurate, and each is rounded once
         assert (np.abs(total) <= 2 * (bound + (2 * (gap + 2 + np.log(classes)) + 40) * U * want)).all()
+
+
+# ------------------------------------------------------------------------------------------
+# outputs that the caller gives
+# ------------------------------------------------------------------------------------------
+def test_given_outputs_that_share_elements_with_an_input_are_refused(env):
+    torch, ops = env
+    gen = torch.Generator().manual_seed(58)
+    n, c = 200, 16
+    wide = randn(torch, gen, n + 1, 3 * c)
+    x, f, free = wide[:n, :c], wide[:n, c:2 * c], wide[:n, 2 * c:]
+    off = torch.tensor([0, n]).cuda()
+    kw = dict(offsets=off, max_len=n)
+    want = ops.gated_scan(x, f, **kw)["y"]
+    for out in (x, f, wide[1:, :c], wide[:n, 1:c + 1], wide[:n, 2 * c - 1:-1], wide[1:, 2 * c - 3:-3], wide.view(-1)[5:5 + n * c].view(n, c)):
+        kept = wide.clone()
+        with pytest.raises(ValueError, match="shares elements"):
+            ops.gated_scan(x, f, out=out, **kw)
+        assert torch.equal(wide, kept)
+    # other columns, other rows, a row that is repeated: apart
+    assert torch.equal(ops.gated_scan(x, f, out=free, **kw)["y"], want)
+    some = dict(offsets=torch.tensor([0, 50]).cuda(), max_len=50)
+    assert torch.equal(ops.gated_scan(x[:50], f[:50], out=wide[100:150, :c], **some)["y"], want[:50])
+    every = torch.empty((100, 2, c), device="cuda")  # every other row
+    every[:, 0] = x[:100]
+    ops.gated_scan(every[:, 0], f[:100], out=every[:, 1], offsets=torch.tensor([0, 100]).cuda(), max_len=100)
+    assert torch.equal(every[:, 1], ops.gated_scan(x[:100], f[:100], offsets=torch.tensor([0, 100]).cuda(), max_len=100)["y"])
+    h = torch.zeros(2 * c, device="cuda")
+    with pytest.raises(ValueError, match="h_last: shares elements with h0"):
+        ops.gated_scan(x, f, h0=h[:c].view(1, c), h_last=h[1:c + 1].view(1, c), **kw)
+    ops.gated_scan(x, f, h0=h[:c].view(1, c), h_last=h[c:].view(1, c), **kw)
+
+
+@pytest.mark.parametrize("width", [24, 256, 700])
+def test_block_norm_in_place_of_an_input(env, width):
+    """r' in the place of the residual, the block's output or the gate, row for row; shifted by a row or a column it is refused."""
+    torch, ops = env
+    gen = torch.Generator().manual_seed(59)
+    rows = 3000
+    y, r, g = (randn(torch, gen, rows + 1, width + 4)[:, :width] for _ in range(3))
+    want = ops.block_norm(y[:rows], r[:rows], g[:rows])
+    for k in range(3):
+        a = [t.clone() for t in (y, r, g)]
+        a[k] = torch.empty((rows + 1, width + 4), device="cuda")[:, :width].copy_(a[k])
+        got = ops.block_norm(*(t[:rows] for t in a), out=a[k][:rows])
+        assert torch.equal(got["residual"], want["residual"]) and torch.equal(got["normed"], want["normed"])
+        with pytest.raises(ValueError, match="shares elements"):
+            ops.block_norm(*(t[:rows] for t in a), out=a[k][1:])
+    with pytest.raises(ValueError, match="shares elements"):
+        ops.block_norm(y[:rows].bfloat16(), r[:rows], out=r.as_strided((rows, width), (width + 4, 1), 1))
