@@ -182,6 +182,56 @@ def test_gated_scan_infinities_go_as_the_definition_says(env, lengths, c, dtype,
 
 
 # ------------------------------------------------------------------------------------------
+# gated_scan: every form against the definition
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype,lengths,c", [
+    ("float32", [9001], 64), ("bfloat16", [9001], 128), ("float16", [9001], 129), ("bfloat16", [4500, 17], 256),  # chunks of whole tiles
+    ("float32", [1000] * 20, 192), ("bfloat16", [200, 64, 900], 512), ("float16", [130, 700], 768)])              # more than one block of full lanes
+def test_gated_scan_whole_tiles_and_blocks_of_channels(env, dtype, lengths, c, reverse):
+    torch, ops = env
+    gen = torch.Generator().manual_seed(60)
+    n, k = sum(lengths), len(lengths)
+    x, f, gy = (randn(torch, gen, n, c, dtype=dtype) for _ in range(3))
+    f = (f.float() * 2 + 3).to(f.dtype)
+    scan_against_the_definition(torch, ops, x, f, lengths, randn(torch, gen, k, c), gy, randn(torch, gen, k, c), reverse)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype,c", [("float32", 64), ("bfloat16", 50), ("float16", 33), ("float32", 6)])
+def test_gated_scan_in_chunks_with_gaps_empty_and_refused_sequences(env, dtype, c, reverse):
+    """begin / end of long, short, empty and refused sequences, divided into chunks, with states and gradients of states."""
+    torch, ops = env
+    from oracle import sequence_ref as ref
+
+    gen = torch.Generator().manual_seed(61)
+    n, max_len = 9000, 5000
+    ranges = [(3000, 8000), (100, 130), (1000, 1000), (-4, 30), (150, 900), (2000, 8900), (8500, 9001), (40, 39), (8999, 9000), (0, 0)]
+    good = [i for i, (b, e) in enumerate(ranges) if 0 <= b <= e <= n and e - b <= max_len]
+    bad = [i for i in range(len(ranges)) if i not in good]
+    assert ops._lib.lib().dc_gated_scan_workspace(n, c, len(ranges), max_len) > 0  # (chunks have maps)
+    x, f, gy = (randn(torch, gen, n, c, dtype=dtype) for _ in range(3))
+    f = (f.float() * 2 + 2).to(f.dtype)
+    h0, gl = randn(torch, gen, len(ranges), c), randn(torch, gen, len(ranges), c)
+    b, e = (torch.tensor([r[i] for r in ranges]).cuda() for i in (0, 1))
+    kw = dict(begin=b, end=e, max_len=max_len, h0=h0, reverse=reverse)
+    r = ops.gated_scan(x, f, save=True, **kw)
+    g = ops.gated_scan_backward(x, f, r["saved"], gy, grad_h_last=gl, **kw)
+    want, bound = ref.gated_scan(host(x), host(f), [ranges[i] for i in good], host(h0)[good], reverse, host(gy), host(gl)[good])
+    covered = ~np.isnan(want["y"][:, 0])
+    inside = torch.from_numpy(covered).cuda()
+    for name, t in (("y", r["y"]), ("grad_x", g["grad_x"]), ("grad_f", g["grad_f"])):
+        check(name, t[inside], want[name][covered], bound[name][covered])
+        assert (t[~inside] == 0).all()
+    for name, t in (("h_last", r["h_last"]), ("grad_h0", g["grad_h0"])):
+        check(name, t[good], want[name], bound[name])
+        assert torch.isnan(t[bad]).all()
+    out = torch.full((n, c), 5.0, device="cuda").to(x.dtype)
+    again = ops.gated_scan(x, f, out=out, **kw)
+    assert (out[~inside] == 5).all() and torch.equal(out[inside], r["y"][inside]) and torch.equal(again["h_last"][good], r["h_last"][good])
+
+
+# ------------------------------------------------------------------------------------------
 # block_norm
 # ------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("act", ["sigmoid", "silu"])
