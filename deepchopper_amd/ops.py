@@ -379,11 +379,12 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, *, offsets: torch.Tensor | None
     counterpart of the long convolution, for reads of any length, with a state to carry on with.
 
     x, f [n_seqs, length, n_channels] dense, or [n_tokens, n_channels] with the sequences at `offsets` int64[n_seqs + 1], or at
-    `begin` / `end` int64[n_seqs] (left-padded rows: first column and end of each).  `h0` f32[n_seqs, n_channels] state to start from; `reverse`: from
-    the sequences' ends.  `h_last` may be given (`h0` itself: a state kept in place while bases stream in); `out` (apart from x and f) keeps
-    what stands in tokens of no sequence, which are zero otherwise.  `max_len`: no sequence is longer (found on the host, with a wait, where it is not
-    given).  A sequence that is, or that leaves the tokens, is refused: NaN in its row of h_last and, with `offsets`, in its rows of y; with
-    `begin` / `end` or a given `out` those stay as tokens of no sequence.  Returns dict(y, h_last, saved: for `gated_scan_backward`, with `save`)."""
+    `begin` / `end` int64[n_seqs] (left-padded rows: first column and end of each); n_seqs * ceil(n_channels / 64) is below 2^20.
+    `h0` f32[n_seqs, n_channels] state to start from; `reverse`: from the sequences' ends.  `h_last` may be given (`h0` itself: a state
+    kept in place while bases stream in); `out` (apart from x and f) keeps what stands in tokens of no sequence, which are zero
+    otherwise.  `max_len`: no sequence is longer (found on the host, with a wait, where it is not given).  A sequence that is, or that
+    leaves the tokens, is refused: NaN in its row of h_last and, with `offsets`, in its rows of y; with `begin` / `end` or a given `out`
+    those stay as tokens of no sequence.  Returns dict(y, h_last, saved: for `gated_scan_backward`, with `save`)."""
     _not_recorded("gated_scan", x, f, h0)
     dev = _device_of("x", x)
     xp, xs = _rows(dev, "x", x)
@@ -392,17 +393,18 @@ def gated_scan(x: torch.Tensor, f: torch.Tensor, *, offsets: torch.Tensor | None
     n, c, seqs, longest, b, e = _scan_shape(dev, x, offsets, begin, end, max_len)
     h0p = _like(dev, "h0", h0, (seqs, c), torch.float32)
     zero_rest = out is None and offsets is not None  # (dense sequences cover every token)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _new_like(x, dtype) if begin is None else torch.zeros(shape, dtype=dtype, device=device)
-        yp, ys = _rows(dev, "out", out, shape, dtype)
-    else:
-        yp, ys = _rows(dev, "out", out, shape, dtype)
+    yp, ys = _rows(dev, "out", out, shape, dtype)
+    if given:
         _apart("out", out, (yp, ys), "x", x, (xp, xs))
         _apart("out", out, (yp, ys), "f", f, (fp, fs))
-    if h_last is None:
+    given = h_last is not None
+    if not given:
         h_last = torch.empty_like(h0) if h0 is not None else x.new_empty((seqs, c), dtype=torch.float32)
     hp = _like(dev, "h_last", h_last, (seqs, c), torch.float32)
-    if h0p is not None and h0p != hp:
+    if given and h0p is not None and h0p != hp:
         _apart("h_last", h_last, (hp, c), "h0", h0, (h0p, c))
     L = _lib.lib()
     saved = x.new_empty(L.dc_gated_scan_saved(n, c), dtype=torch.float32) if save else None
