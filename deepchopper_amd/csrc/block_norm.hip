@@ -8,8 +8,9 @@
 // the forward pass is read back: r', u and both norms' statistics cost less to take again from the inputs than to load.
 // The vectors' gradients: every lane sums its own columns over the rows of its workgroup, the workgroups' sums go to the workspace
 // and are added in order by a second kernel (no atomics).
-// Measured (a large copy: 4.7 TB/s): 524 288 x 256 bf16 on an fp32 residual forward 382 us = 4.9 TB/s, 65 537 x 1000 bf16 forward 137 us =
-// 4.8 TB/s, backward 262 us = 4.0 TB/s; bf16 backward is bound by vector work, 55 operations a column and four exchanges a row.
+// Measured (a large copy: 4.7 TB/s): 524 288 x 256 bf16 on an fp32 residual forward 384 us = 4.9 TB/s, backward 592 us = 5.0 TB/s (fp32 throughout
+// 562 us = 4.8 TB/s, 851 us = 5.0 TB/s); 65 537 x 1000 bf16 forward 137 us = 4.8 TB/s, backward 266 us = 3.9 TB/s: bound by vector work, 55
+// operations a column and four exchanges a row.  Beyond 4 096 columns the backward pass spills: 8 192 x 8 192 bf16 824 us = 1.3 TB/s.
 #include <type_traits>
 
 #include "elem_io.h"

@@ -16,8 +16,10 @@
 // a 64-token tile (narrow batches: 16 or 32 lanes a row and 32 or 16 such groups), keep them in registers, pass each other their
 // maps through LDS and run the steps again from the state they then know.  Where sequences and channels alone do not fill the chip,
 // a sequence is divided into chunks: a first kernel reads each chunk for its map alone, the second starts from the composed maps.
-// Measured (a large copy: 4.7 TB/s): 1 024 sequences of 500 - 1 500 x 256 bf16 339 us = 4.6 TB/s; 255 of 20 - 4 001 x 768 fp16 forward 588 us =
-// 4.0 TB/s, backward 960 us = 4.1 TB/s (vector work, 80 - 85 % busy); one of 100 001 x 256 fp32 44 + 56 us and 39 + 91 us backward.
+// Measured (a large copy: 4.7 TB/s): 1 024 sequences of 500 - 1 500 x 256 bf16 342 us = 4.6 TB/s; 255 of 20 - 4 001 x 768 fp16 forward 571 us =
+// 4.2 TB/s, backward 965 us = 4.1 TB/s (vector work, 81 % busy both); one of 100 001 x 256 fp32 43 + 55 us and 37 + 94 us backward.  Channels
+// that do not fill the lanes cost their idle ones and a check a row: 255 of 20 - 4 001 x 129 fp16 445 + 651 us, x 128 220 + 302 us.  Up to 16
+// tokens: 16 384 x 16 x 256 bf16 forward 87 us = 4.6 TB/s, backward 225 us = 3.0 TB/s.
 #include <initializer_list>
 #include <type_traits>
 
@@ -943,7 +945,7 @@ extern "C" int64_t dc_gated_scan_saved(int64_t n_tokens, int32_t n_channels) {
 
 extern "C" int64_t dc_gated_scan_workspace(int64_t n_tokens, int32_t n_channels, int32_t n_seqs, int64_t max_len) {
   if (n_tokens <= 0 || n_channels <= 0 || n_seqs <= 0 || max_len <= dc::kShort) return 0;
-  // maps and starts of whichever division the alignment of the tensors allows
+  // maps and starts of either division: with one or with two channels a lane (by the element type, which is not said here)
   int64_t most = 0;
   for (int v = 1; v <= 2; ++v) {
     const dc::Plan p = dc::scan_plan(n_tokens, n_channels, n_seqs, max_len, v);

@@ -11,9 +11,9 @@
 // Top alternatives of a walk: the n-th largest of the lanes' (or quads') maxima bounds the n-th largest class from below, so one comparison
 // a class against that bound leaves a few candidates, which are collected in LDS and ranked by counting; the bound only rises from
 // there on.  Ties go to the lower class throughout: candidates are ordered by (logit, class).
-// Measured (a large copy: 4.7 TB/s): 2 050 048 x 2 fp32 with one alternative 12.5 us (47 MB); 4 096 x 100 003 bf16 forward 188 us = 4.4 TB/s,
-// backward 272 us = 6 TB/s; 16 384 x 4 096 bf16 with four alternatives 50 us (vector work, 22 operations a class); 5 x 50 257 fp16 with
-// twenty 9.3 + 6.7 us (latency).
+// Measured (a large copy: 4.7 TB/s): 2 050 048 x 2 fp32 with one alternative 13.6 us (47 MB); 4 096 x 100 003 bf16 forward 188 us = 4.4 TB/s,
+// backward 270 us = 6 TB/s; 16 384 x 4 096 bf16 with four alternatives 50 us (vector work, 22 operations a class); 5 x 50 257 fp16 with
+// twenty 9.4 + 5.9 us (latency).  A piece is worked in full whatever of it the row fills: 16 384 x 600 bf16 16.1 us, as x 1 024.
 #include <type_traits>
 
 #include "elem_io.h"
@@ -640,7 +640,9 @@ __global__ __launch_bounds__(256) void many_classes_backward_kernel(const T* log
   }
 }
 
-// How a forward call is divided beyond DC_STATS_FROM classes: about four wavefronts a SIMD, slices of at least 1 024 classes.
+// How a forward call is divided beyond DC_STATS_FROM classes: about four wavefronts a SIMD, slices of at least 1 024 classes, none from 2 048
+// rows on.  Calls in bf16, a wavefront a row against slices: 512 x 100 003 53 / 27 us, 1 024 x 100 003 54 / 42 us, 2 047 x 100 003 81 / 84 us,
+// 2 048 x 100 003 81 / 84 us, 512 x 32 768 17 / 14 us; up to 8 192 classes the second launch is what counts (512 x 8 192 10.4 / 14.6 us).
 int slices_of(int64_t n_rows, int32_t n_classes) {
   if (n_rows <= 0 || n_rows >= 2048 || n_classes < DC_STATS_FROM) return 1;
   int64_t s = (4096 + n_rows - 1) / n_rows;
@@ -649,7 +651,9 @@ int slices_of(int64_t n_rows, int32_t n_classes) {
 }
 
 // Up to 512 classes: classes a lane and lanes a row, as a power of two.  4 neighbouring classes a lane and up to 16 lanes; then more of
-// them a lane, so that four (two) rows share a wavefront's reductions.
+// them a lane, so that four (two) rows share a wavefront's reductions.  4, 8 and 16 a lane, fp32, forward + backward: 524 352 x 16
+// 13.6 + 17.1, 10.7 + 15.6 and 10.6 + 20.2 us; 400 000 x 64 34 + 43, 24 + 34 and 22 + 41 us; 300 000 x 128 51 + 76, 35 + 58 and 30 + 68 us: 8
+// from 5 classes on are faster than the 4 taken here.
 int few_classes_a_lane(int32_t n_classes) { return n_classes <= 2 ? 2 : n_classes <= 64 ? 4 : n_classes <= 128 ? 8 : 16; }
 int lane_bits_of(int32_t n_classes) {
   int bits = 0;

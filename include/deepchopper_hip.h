@@ -456,7 +456,8 @@ int dc_token_logprobs_backward(void* stream, const void* d_logits, int32_t dtype
  *               2^-126 are 0, but an infinite state (or gradient) stays infinite until it meets the other infinity: NaN
  *  d_begin, d_end: int64[n_seqs] on the device, sequence s = tokens [begin[s], end[s]) (offsets of a packed batch: pass
  *               offsets and offsets + 1), which may not overlap, or both NULL: n_seqs dense sequences of max_len tokens
- *  max_len    : no sequence is longer (host value: it shapes the launch)
+ *  max_len    : no sequence is longer (host value: it shapes the launch);  n_channels <= 2^24 and
+ *               n_seqs * ceil(n_channels / 64) < 2^20, or the call is refused
  *  d_h0       : float[n_seqs, n_channels] state before the first token, or NULL (zeros)
  *  d_y        : [n_tokens, n_channels], not overlapping the inputs; tokens of no sequence are left untouched, or with
  *               zero_rest != 0 (packed sequences: begin ascending, end[s] = begin[s + 1]) those in front of begin[0] and from
@@ -489,7 +490,8 @@ int dc_gated_scan_backward(void* stream, int32_t dtype, const void* d_x, int64_t
 /* What stands between two blocks: the norm behind one, its gate and residual scale, and the norm in front of the next.
  *   u = norm(y) * post_w + post_b  (post_norm = 0: u = y)     v = act(gate) * u  (d_gate NULL: v = u)
  *   r' = residual + scale * v                                 n = norm(r') * pre_w + pre_b
- *   norm(x) = (x - mean) / sqrt(var + eps) (DC_NORM_LAYER) or x / sqrt(mean(x^2) + eps) (DC_NORM_RMS)
+ *   norm(x) = (x - mean) / sqrt(var + eps) (DC_NORM_LAYER) or x / sqrt(mean(x^2) + eps) (DC_NORM_RMS), its sums in fp32: of a
+ *   row whose squares add up to more than 3.4e38 (values of 1.8e19 / sqrt(width)) it is 0 or NaN
  *  dtype          : of y, gate and n;  residual_dtype: of residual and r', DC_DTYPE_F32 or dtype.  n is taken of r' in fp32,
  *                   before r' is rounded
  *  d_y            : NULL: no block in front (r' = residual; the first norm of a model);  d_residual NULL: r' = scale * v
