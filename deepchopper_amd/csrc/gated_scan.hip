@@ -608,7 +608,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_kernel(ScanArgs a, cons
   const int64_t sc = (int64_t)at.s * a.n_channels + at.channel;
   const int64_t j0 = at.chunk * a.chunk, j1 = j0 + a.chunk < q.len ? j0 + a.chunk : q.len;
   if (j0 >= q.len && at.chunk > 0) return;
-  if (threadIdx.x < 64) lost[threadIdx.x] = 0;  // (set behind the last tile; without a tile there is nothing to walk again)
+  if (threadIdx.x < 64) lost[threadIdx.x] = 0;  // (set behind the chunks' barriers or the last tile's; with neither there is nothing to walk)
   float carry[V];
   if (maps) {
     compose_chunks<V>(a, at, maps, 0, 1, at.chunk, lds[0], carry);
@@ -724,7 +724,7 @@ __global__ __launch_bounds__(kThreads, 4) void scan_tile_backward_kernel(ScanArg
   const int64_t sc = (int64_t)at.s * a.n_channels + at.channel;
   const int64_t j0 = at.chunk * a.chunk, j1 = j0 + a.chunk < q.len ? j0 + a.chunk : q.len;
   if (j0 >= q.len && at.chunk > 0) return;
-  if (threadIdx.x < 64) lost[threadIdx.x] = 0;  // (set behind the last tile; without a tile there is nothing to walk again)
+  if (threadIdx.x < 64) lost[threadIdx.x] = 0;  // (set behind the chunks' barriers or the last tile's; with neither there is nothing to walk)
   float carry[V];  // a_t g_t of the token behind
   if (maps) {
     const int last = q.len > 0 ? (int)((q.len - 1) / a.chunk) : 0;
